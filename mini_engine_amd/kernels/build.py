@@ -1,8 +1,8 @@
 """Compile the HIP sources for gfx950 into shared libraries and find them again.
 
-Two kinds of library: ``libme_core.so`` (every kernel that takes its sizes at run
+Kinds of library: ``libme_core.so`` (every kernel that takes its sizes at run
 time) and ``libme_attn_d<D>.so`` (the MFMA attention kernels, specialised per
-head size); beside them ``me_calls.so``, a Python module through which their entry points are called. A library is rebuilt when the hash of its sources and flags differs
+head size; ``libme_attn8_d<D>.so`` those over an 8-bit cache); beside them ``me_calls.so``, a Python module through which their entry points are called. A library is rebuilt when the hash of its sources and flags differs
 from the one recorded beside it. Libraries live in ``mini_engine_amd/lib`` when
 that folder can be written, else in a per-user folder under the temp directory.
 """
@@ -34,14 +34,16 @@ HIPCC_FLAGS = [
 ]
 CORE_SOURCES = ["elementwise.hip", "rope_kv.hip", "attention_simple.hip",
                 "gemm.hip", "gemm_f32.hip", "gemm_mid.hip", "gemm_tile.hip", "gemm_library.hip", "sampling.hip", "recurrent.hip", "parallel.hip", "moe.hip", "hybrid.hip", "linear_chunks.hip", "latent.hip",
-                "streams.hip"]
+                "streams.hip", "kv_e4m3.hip"]
 ATTN_SOURCE = "attention_mfma.hip"
-HEADERS = ["common.h", "errors.inc", "sampling.h", "chunks.h"]
+ATTN_E4M3_SOURCE = "attention_e4m3.hip"
+HEADERS = ["common.h", "errors.inc", "sampling.h", "chunks.h", "e4m3.h"]
 CALLS_SOURCE = "calls.cpp"
 # Head sizes that build_all() compiles ahead of use; any other multiple of 16 up to 512 is compiled when a model first needs it.
 DEFAULT_HEAD_DIMS = (16, 32, 48, 64, 80, 128, 256)
 CAPPED_HEAD_DIMS = (32, 64, 128)          # ... of the variant with a cap on the scores
 DISTANCE_HEAD_DIMS = (16, 32, 48, 64, 128)          # ... of the variant with slopes times distances
+E4M3_HEAD_DIMS = (16, 32, 48, 64, 80, 128, 256)          # ... of the attention over an 8-bit cache
 
 _locks: dict = {}
 _locks_guard = threading.Lock()
@@ -205,6 +207,13 @@ def attention_library(head_dim: int, force: bool = False, score_cap: bool = Fals
     return _ensure(f"libme_attn_d{head_dim}{'c' * score_cap}{'d' * distance}.so", [ATTN_SOURCE], flags, force)
 
 
+def attention_e4m3_library(head_dim: int, force: bool = False) -> str:
+    """The attention kernels over a cache of e4m3 numbers for one head size."""
+    if head_dim % 16 or not 16 <= head_dim <= 256:
+        raise BuildError(f"attention over an 8-bit cache needs a head size that is a multiple of 16 in 16..256, got {head_dim}")
+    return _ensure(f"libme_attn8_d{head_dim}.so", [ATTN_E4M3_SOURCE], [f"-DME_HEAD_DIM={head_dim}"], force)
+
+
 def calls_library(force: bool = False) -> str | None:
     """The Python module of csrc/calls.cpp, for the interpreter that runs; None where it is not built and cannot be (no compiler, no
     headers of Python, a machine with another calling convention)."""
@@ -245,4 +254,5 @@ def build_all(head_dims=DEFAULT_HEAD_DIMS, force: bool = True) -> list:
         libs += list(pool.map(lambda d: attention_library(d, force=force), head_dims))
         libs += list(pool.map(lambda d: attention_library(d, force=force, score_cap=True), CAPPED_HEAD_DIMS))
         libs += list(pool.map(lambda d: attention_library(d, force=force, distance=True), DISTANCE_HEAD_DIMS))
+        libs += list(pool.map(lambda d: attention_e4m3_library(d, force=force), E4M3_HEAD_DIMS))
     return [lib for lib in libs if lib]

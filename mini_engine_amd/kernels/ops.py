@@ -125,6 +125,7 @@ _CORE_PROTOS = {
     "me_decay_rows_recurrence": [P, L, P, L, P, L, P, L, P, L, I, P, P, P, P, L, P, P, P, I, I, I, I, I, I, I, F, F, I, L, P, P],
     "me_linear_chunks": [P, L, P, L, P, L, P, L, P, P, P, P, P, L, P, P, P, I, I, I, I, I, I, L, P, L, P],
     "me_reset_rows": [P, P, P, P, I, P, I, L, P],
+    "me_append_e4m3": [P, L, P, P, P, F, P, L, L, P, P, P, P, P, P, L, L, I, I, I, I, I, P],
     "me_sample": [P, L, P, P, P, P, I, I, P],
     "me_sample_static": [P, L, P, P, P, I, I, P],
 }
@@ -132,6 +133,11 @@ _ATTN_PROTOS = {
     "me_attn_prefill": [P, L, P, L, P, P, P, I, P, P, I, L, I, I, I, F, I, I, I, I, I, I, P, P, I, F, P, P, P, P],
     "me_attn_decode": [P, L, P, L, P, P, P, I, P, I, I, I, I, F, I, I, I, P, I, F, P, P, P, P, L, P],
     "me_attn_decode_fused": [P, L, P, L, P, P, F, P, I, P, P, P, I, P, I, I, I, I, I, F, I, I, I, P, I, F, P, P, P, I, P, L, P],
+}
+
+_ATTN_E4M3_PROTOS = {
+    "me_attn8_decode": [P, L, P, L, P, P, P, P, L, P, I, I, P, I, I, I, I, F, I, I, I, I, P, P, P],
+    "me_attn8_prompt": [P, L, P, L, P, P, P, P, L, P, I, I, P, P, L, I, I, I, I, F, I, I, I, I, P, P, P],
 }
 
 _core: _Lib | None = None
@@ -162,6 +168,18 @@ def attn_lib(head_dim: int, score_cap: bool = False, distance: bool = False) -> 
         if lib.cdll.me_attn_head_dim() != head_dim:
             raise KernelError(f"{lib.path} was built for head size {lib.cdll.me_attn_head_dim()}, not {head_dim}")
         _attn[key] = lib
+    return lib
+
+
+def attn_e4m3_lib(head_dim: int) -> _Lib:
+    lib = _attn.get(("e4m3", head_dim))
+    if lib is None:
+        _require_gpu()
+        lib = _Lib(build.attention_e4m3_library(head_dim), _ATTN_E4M3_PROTOS)
+        lib.cdll.me_attn8_head_dim.restype = c_int
+        if lib.cdll.me_attn8_head_dim() != head_dim:
+            raise KernelError(f"{lib.path} was built for head size {lib.cdll.me_attn8_head_dim()}, not {head_dim}")
+        _attn[("e4m3", head_dim)] = lib
     return lib
 
 
@@ -346,6 +364,43 @@ class MemoryReads:
 
     def __init__(self, y, dot, floor, gates: SoftGates):
         self.y, self.dot, self.floor, self.gates = y, dot, floor, gates
+
+
+class PagesE4M3:
+    """One layer's pages of an 8-bit cache: k [pages, Hkv, page, D] and v [pages, Hkv, D, page] of e4m3 numbers
+    (torch.float8_e4m3fn), k_scales and v_scales [pages, Hkv, page / 16] bytes: the power of two of each block of 16 tokens and
+    head, with 127 added. What a place stands for is its number times the block's power (a bfloat16 number, exactly). A page has
+    a power of two of tokens, 16 or more. An infinity is stored as NaN, which e4m3 has, and neither counts for a block's power."""
+
+    BLOCK = 16
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor):
+        self.k, self.v, self.k_scales, self.v_scales = k, v, k_scales, v_scales
+
+    def check(self, what: str, Hkv: int, D: int, page: int) -> int:
+        """Raises unless the tensors are such pages; returns how many there are."""
+        _check(page >= self.BLOCK and page & (page - 1) == 0, f"{what}: a page has a power of two of tokens, 16 or more, not {page}")
+        _check(D % 16 == 0 and 16 <= D <= 256, f"{what}: the head size must be a multiple of 16 up to 256, not {D}")
+        k, v, n = self.k, self.v, self.k.shape[0] if self.k.dim() else 0
+        if not (n >= 1 and k.shape == (n, Hkv, page, D) and v.shape == (n, Hkv, D, page) and k.dtype == v.dtype == torch.float8_e4m3fn
+                and k.is_contiguous() and v.is_contiguous()):
+            raise KernelError(f"{what}: pages must be contiguous e4m3 numbers, K [pages, Hkv, page, D] and V [pages, Hkv, D, page]")
+        for t in (self.k_scales, self.v_scales):
+            _check(t.dtype == torch.uint8 and t.shape == (n, Hkv, page // self.BLOCK) and t.is_contiguous(),
+                   f"{what}: the blocks' powers must be contiguous uint8 [pages, Hkv, page / 16]")
+        return n
+
+    def tensors(self) -> tuple:
+        return self.k, self.v, self.k_scales, self.v_scales
+
+
+def _check_device(what: str, *tensors) -> None:
+    """All on the GPU that launches go to: the kernels run on the current device's current stream."""
+    _require_gpu()
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and not (t.is_cuda and t.device.index == here):
+            raise KernelError(f"{what}: every tensor must be on the current GPU (cuda:{here}), got one on {t.device}")
 
 
 class HipBackend:
@@ -624,6 +679,94 @@ class HipBackend:
                          int(bool(values_are_keys)), _ptr(inside), 0 if inside is None else inside.stride(0), _stream())
         if head_gate is not None and inside is None:
             self.head_gate(out, head_gate, Hq, D)
+        return out
+
+    # -- the 8-bit cache -------------------------------------------------------------------
+    def qk_norm_rope_store_e4m3(self, rows, q_weight, k_weight, eps, table, positions, slots, pages: PagesE4M3, Hq: int, Hkv: int, D: int,
+                                page: int, position_bound: int = 0, values_are_keys: bool = False) -> torch.Tensor:
+        """`qk_norm_rope_store` into an 8-bit cache: per-head RMSNorm of q and k (weights float32 [D] or None), rotation by `table`
+        (or None), keys and values to their pages in e4m3, each rounded once from its float32 result. The rows [T, (Hq+2Hkv)*D]
+        (values_are_keys: [T, (Hq+Hkv)*D], a value is its key as projected) stay as they are; returns the queries, bfloat16
+        [T, Hq*D] (Hq may be 0: rows of keys and values alone).
+
+        A block (16 places of a page, one head) has the least power of two under which the largest of its numbers fits. Rows of one
+        block stand next to each other in the order of their slots, as a step's requests bring them; then a call that begins a block
+        at its place 0 opens it anew, any other keeps what stands in front of its first place: the power never falls, and where it
+        grows those numbers are rounded again (exactly, unless they fall below e4m3's smallest normal number). Places behind the last
+        one written hold nothing: they keep their bytes, which a grown power leaves without meaning. Rows of one block that follow each
+        other in another order are taken as calls one after the other; a block whose rows stand apart in one call holds either of them.
+        slots below 0 or beyond the pages are skipped. (reference models/qwen3.py:34-36, layers/rotary_embedding.py:20-25,
+        csrc/kv_cache.cu:10-31, whose cache has the activations' type.)"""
+        what = "qk_norm_rope_store_e4m3"
+        _check(rows.dtype == torch.bfloat16, f"{what}: rows must be bfloat16, got {rows.dtype}")
+        T = rows.shape[0]
+        width = (Hq + (1 if values_are_keys else 2) * Hkv) * D
+        if not (rows.dim() == 2 and rows.stride(1) == 1 and rows.shape[1] == width and (T <= 1 or rows.stride(0) >= width)):
+            raise KernelError(f"{what}: rows must be [T, {width}] with unit inner stride, got {tuple(rows.shape)}")
+        _check(Hq >= 0 and Hkv >= 1, f"{what}: bad head counts")
+        n = pages.check(what, Hkv, D, page)
+        for w in (q_weight, k_weight):
+            _check(w is None or (w.dtype == torch.float32 and w.shape == (D,) and w.is_contiguous()), f"{what}: norm weights must be float32 [D]")
+        _check((q_weight is None) == (k_weight is None), f"{what}: give both norm weights or neither")
+        if table is not None:
+            _check(table.dtype == torch.float32 and table.is_contiguous() and table.dim() == 3 and table.shape[1:] == (D // 2, 2),
+                   f"{what}: rotary table must be float32 [P, D/2, 2]")
+        _check(_is_i32(positions, T) and _is_i32(slots, T), f"{what}: positions and slots must be int32 [T]")
+        _check_device(what, rows, q_weight, k_weight, table, positions, slots, *pages.tensors())
+        q = torch.empty((T, Hq * D), dtype=rows.dtype, device=rows.device)
+        core().call("me_append_e4m3", rows.data_ptr(), max(rows.stride(0), width), q.data_ptr(), _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(table),
+                    0 if table is None else table.shape[0], int(position_bound), positions.data_ptr(), slots.data_ptr(), pages.k.data_ptr(),
+                    pages.v.data_ptr(), pages.k_scales.data_ptr(), pages.v_scales.data_ptr(), n, T, Hq, Hkv, D, page,
+                    int(bool(values_are_keys)), _stream())
+        return q
+
+    def paged_attention_e4m3(self, q, pages: PagesE4M3, page: int, block_tables, context_lens, seq_of_token, positions, prefill_cu,
+                             num_decodes: int, max_decode_context: int, scale: float, window: int | None, Hq: int, Hkv: int, D: int,
+                             max_prefill_context: int = 0, even_contexts: bool = False, chunk: int | None = None, sinks=None) -> torch.Tensor:
+        """`paged_attention` over an 8-bit cache, its arguments with the meanings they have there: causal attention of this step's
+        tokens (`num_decodes` single tokens first, then the requests whose new tokens `prefill_cu` counts) over the paged keys of
+        their requests, under a window, a block mask `chunk` or neither, with learned `sinks` (float32 [Hq]) or none. A request's
+        new tokens are its last ones; keys in table entries that hold no page are not seen, a token that sees no key gets zeros, and
+        rows behind the last request are left as they are allocated. bfloat16 queries, head sizes in steps of 16 up to 256, pages of
+        a power of two from 16 on. Returns [T, Hq*D]. (reference layers/attention.py:63-76, over a cache of the activations' type.)"""
+        what = "paged_attention_e4m3"
+        T, B = q.shape[0], context_lens.numel()
+        _check(q.dtype == torch.bfloat16, f"{what}: queries must be bfloat16, got {q.dtype}")
+        _check(q.dim() == 2 and q.shape[1] == Hq * D and q.stride(1) == 1 and (T <= 1 or q.stride(0) >= Hq * D),
+               f"{what}: q must be [T, Hq*D], unit inner stride")
+        n = pages.check(what, Hkv, D, page)
+        _check(block_tables.dim() == 2 and block_tables.dtype == torch.int32 and block_tables.stride(1) == 1 and block_tables.shape[0] >= B
+               and block_tables.shape[1] >= 1, f"{what}: block tables must be int32 [B, MB]")
+        _check(_is_i32(context_lens) and _is_i32(seq_of_token, T) and _is_i32(positions, T), f"{what}: metadata must be int32")
+        _check(0 <= num_decodes <= B and num_decodes <= T, f"{what}: bad decode count")
+        _check(not (window and chunk), f"{what}: a window and a block mask exclude each other")
+        _check((window or 0) >= 0 and (chunk or 0) >= 0, f"{what}: a window or a block must not be negative")
+        _check(sinks is None or (sinks.dtype == torch.float32 and sinks.shape == (Hq,) and sinks.is_contiguous()), f"{what}: sinks must be float32 [Hq]")
+        _check(T == num_decodes or (B > num_decodes and prefill_cu is not None and _is_i32(prefill_cu, B - num_decodes + 1)),
+               f"{what}: prefill_cu must be int32 [B-Dn+1]")
+        _check_device(what, q, block_tables, context_lens, prefill_cu, sinks, *pages.tensors())
+        out = torch.empty((T, Hq * D), dtype=q.dtype, device=q.device)
+        if T == 0:
+            return out
+        lib, span = attn_e4m3_lib(D), int(window or chunk or 0)      # no query sees more keys than `span` (0: all of them)
+        rows = max(q.stride(0), Hq * D)
+        pools = (pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scales.data_ptr(), pages.v_scales.data_ptr(), n)
+        tables = (block_tables.stride(0) if block_tables.shape[0] > 1 else block_tables.shape[1], block_tables.shape[1])
+        if num_decodes > 0:
+            part, parts = decode_partitions_e4m3(num_decodes, Hq, Hkv, max_decode_context, span)
+            # (from torch's allocator, which knows the stream and a capture's memory: calls on two streams never share it)
+            scratch = torch.empty(num_decodes * Hq * parts * (D + 2), dtype=torch.float32, device=q.device) if parts > 1 else None
+            lib.call("me_attn8_decode", q.data_ptr(), rows, out.data_ptr(), Hq * D, *pools, block_tables.data_ptr(), *tables,
+                     context_lens.data_ptr(), num_decodes, Hq, Hkv, page, float(scale), int(window or 0), int(chunk or 0), part, parts,
+                     _ptr(scratch), _ptr(sinks), _stream())
+        if T > num_decodes:
+            Tp = T - num_decodes
+            part, parts = prompt_partitions_e4m3(Tp, B - num_decodes, Hq, Hkv, D, max_prefill_context or block_tables.shape[1] * page, span)
+            scratch = torch.empty(Tp * Hq * parts * (D + 2), dtype=torch.float32, device=q.device) if parts > 1 else None
+            lib.call("me_attn8_prompt", q.data_ptr() + num_decodes * rows * 2, rows, out.data_ptr() + num_decodes * Hq * D * 2, Hq * D, *pools,
+                     block_tables.data_ptr() + num_decodes * tables[0] * 4, *tables, context_lens.data_ptr() + num_decodes * 4,
+                     prefill_cu.data_ptr(), Tp, B - num_decodes, Hq, Hkv, page, float(scale), int(window or 0), int(chunk or 0), part, parts,
+                     _ptr(scratch), _ptr(sinks), _stream())
         return out
 
     # -- matrix products -----------------------------------------------------------------
@@ -1479,6 +1622,26 @@ def _scratch(num_floats: int, device, use: str = "decode") -> torch.Tensor:
     return buf
 
 
+def decode_partitions_e4m3(num_seqs: int, Hq: int, Hkv: int, max_context: int, span: int = 0) -> tuple:
+    """(keys per partition, partitions) of a launch of single tokens over an 8-bit cache."""
+    keys = max(1, min(max_context, span + 63) if span else max_context)
+    base = num_seqs * Hkv * -(-(Hq // Hkv) // 16)
+    parts = max(1, min(-(-512 // base), -(-keys // 256)))
+    part = -(-keys // (parts * 256)) * 256
+    return part, -(-keys // part)
+
+
+def prompt_partitions_e4m3(tokens: int, num_seqs: int, Hq: int, Hkv: int, D: int, max_context: int, span: int = 0) -> tuple:
+    """(keys per partition, partitions) of a launch of prompt portions over an 8-bit cache."""
+    keys = max(1, min(max_context, span + 64 + 63) if span else max_context)
+    groups = (tokens * (Hq // Hkv) // 64 + 1) * Hkv
+    parts = max(1, min(-(-512 // groups), keys // 512))
+    if parts == 1:
+        return 0, 1
+    part = -(-keys // (parts * 64)) * 64
+    return part, -(-keys // part)
+
+
 def prefill_col_tiles(max_context: int, window: int, num_tokens: int, Hq: int, D: int = 128) -> int:
     """Column tiles (of 16 (token, head) pairs) per wave of the prefill kernel: 2 halves the reads of keys and
     values per product but needs twice the columns per workgroup, so it is for launches with many columns (32,768
@@ -2259,6 +2422,8 @@ def qk_norm_rope_store(*a, **k): return backend().qk_norm_rope_store(*a, **k)
 def store_kv(*a, **k): return backend().store_kv(*a, **k)
 def paged_attention(*a, **k): return backend().paged_attention(*a, **k)
 def decode_step_attention(*a, **k): return backend().decode_step_attention(*a, **k)
+def qk_norm_rope_store_e4m3(*a, **k): return backend().qk_norm_rope_store_e4m3(*a, **k)
+def paged_attention_e4m3(*a, **k): return backend().paged_attention_e4m3(*a, **k)
 def linear(*a, **k): return backend().linear(*a, **k)
 def silu_mul_linear(*a, **k): return backend().silu_mul_linear(*a, **k)
 def norm_linear(*a, **k): return backend().norm_linear(*a, **k)

@@ -1,0 +1,429 @@
+"""The 8-bit cache's operators on the GPU against their plain forms in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from e4m3_cases import (BLOCK, LEAST, PlainPages, Step, attend, attention_bound, empty_pages, mild_pages, normed_rotated, place_bound, power_for,
+                        random_pages, rotation)
+from mini_engine_amd.kernels import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+EPS = 1e-5
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _rows(T, Hq, Hkv, D, gen, gap=0, offset=0, values_are_keys=False):
+    """Packed rows, `gap` columns behind each and `offset` in front of the first: (the view, on the GPU; float64, on the CPU)."""
+    width = (Hq + (1 if values_are_keys else 2) * Hkv) * D
+    x = torch.randn(T, width, generator=gen) * torch.exp(torch.randn(T, 1, generator=gen))
+    flat = torch.zeros(T * (width + gap) + offset, dtype=torch.bfloat16)
+    view = flat[offset:].view(T, width + gap)[:, :width]
+    view.copy_(x)
+    on_gpu = flat.to(DEV)[offset:].view(T, width + gap)[:, :width]
+    return on_gpu, view.double()
+
+
+def _append_plain(rows, step, plain, Hq, Hkv, D, qw, kw, table, values_are_keys=False):
+    heads = rows.view(step.T, -1, D)
+    q = normed_rotated(heads[:, :Hq], qw, EPS, table, step.positions)
+    k = normed_rotated(heads[:, Hq:Hq + Hkv], kw, EPS, table, step.positions)
+    v = heads[:, Hq:Hq + Hkv] if values_are_keys else heads[:, Hq + Hkv:]
+    plain.place(k, v, step.slots.tolist())
+    return q, k, v
+
+
+def _check_append(rows, q, pages, plain, before, step, exact_k, exact_v, exact_q, values_exact=True):
+    T = step.T
+    got, stored = PlainPages.of(pages), [t for t in range(T) if step.slots[t] >= 0]
+    assert ((q.cpu().double().view(T, -1) - exact_q.reshape(T, -1)).abs() <= (2.0 ** -8 + 2e-6) * exact_q.reshape(T, -1).abs() + 1e-6 * exact_q.abs().max()).all()
+    assert torch.equal(got.kp, plain.kp) and torch.equal(got.vp, plain.vp)
+    assert torch.equal(got.v, plain.v) or not values_exact
+    # keys: half a step of what they round, wherever the rounding falls
+    k_now, _ = got.numbers()
+    for t in stored:
+        pg, off = divmod(int(step.slots[t]), plain.page)
+        bound = place_bound(exact_k[t], got.kp[pg, :, off // BLOCK][:, None]) + 1e-6 * exact_k[t].abs().max()
+        assert ((k_now[pg, :, off] - exact_k[t]).abs() <= bound).all()
+    # places that the call did not write keep their bytes, or are the block's numbers rounded again
+    written = torch.zeros(plain.k.shape[0], plain.page, dtype=torch.bool)
+    for t in stored:
+        written[int(step.slots[t]) // plain.page, int(step.slots[t]) % plain.page] = True
+    keep = ~written[:, None, :, None].expand_as(got.k)
+    assert torch.equal(got.k[keep], plain.k[keep])
+
+
+HEADS = [(16, 8, 128), (4, 2, 32), (6, 2, 16), (8, 8, 80), (5, 1, 48), (3, 3, 256), (8, 2, 64), (2, 1, 144)]
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", HEADS)
+@pytest.mark.parametrize("page", [16, 64])
+def test_append_mixed_step(Hq, Hkv, D, page):
+    """Single tokens at every kind of place, a padding row, portions that begin and end inside blocks, out of strided rows."""
+    gen = _gen(D + page)
+    step = Step([(1, 0), (1, 5), (1, 15), (1, 16), (1, -1), (1, 33), (1, 200), (2, 0), (40, 7), (16, 16), (33, 100)], page, gen)
+    pages = random_pages(step.pages, Hkv, D, page, gen)
+    plain = PlainPages.of(pages)
+    rows, rows64 = _rows(step.T, Hq, Hkv, D, gen, gap=24)
+    qw, kw = 1 + 0.2 * torch.randn(D, generator=gen), torch.exp(torch.randn(D, generator=gen))
+    table = rotation(256, D)
+    kept = rows.clone()
+    q = ops.qk_norm_rope_store_e4m3(rows, qw.to(DEV), kw.to(DEV), EPS, table.to(DEV), step.positions.to(DEV), step.slots.to(DEV), pages, Hq, Hkv, D,
+                                    page, position_bound=256)
+    eq, ek, ev = _append_plain(rows64, step, plain, Hq, Hkv, D, qw, kw, table)
+    _check_append(rows, q, pages, plain, None, step, ek, ev, eq)
+    assert torch.equal(rows, kept)
+
+
+@pytest.mark.parametrize("T,before", [(257, 0), (300, 9), (1000, 3), (2049, 0)])
+def test_append_long_portion(T, before):
+    """More rows than a wave looks at, whole blocks and their ends, beside single tokens."""
+    Hq, Hkv, D, page = 4, 2, 64, 32
+    gen = _gen(T)
+    step = Step([(1, 40), (1, 16), (T, before), (T // 3, 0)], page, gen)
+    pages = random_pages(step.pages, Hkv, D, page, gen)
+    plain = PlainPages.of(pages)
+    rows, rows64 = _rows(step.T, Hq, Hkv, D, gen)
+    table = rotation(4096, D)
+    w = torch.ones(D)
+    q = ops.qk_norm_rope_store_e4m3(rows, w.to(DEV), w.to(DEV), EPS, table.to(DEV), step.positions.to(DEV), step.slots.to(DEV), pages, Hq, Hkv, D, page)
+    eq, ek, ev = _append_plain(rows64, step, plain, Hq, Hkv, D, w, w, table)
+    _check_append(rows, q, pages, plain, None, step, ek, ev, eq)
+
+
+@pytest.mark.parametrize("norm,turn,same", [(False, True, False), (True, False, False), (False, False, False), (True, True, True), (False, False, True)])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_append_options(norm, turn, same, offset):
+    """Without a norm, a rotation, values of their own; rows that begin at an odd address."""
+    Hq, Hkv, D, page = 4, 2, 32, 16
+    gen = _gen(7)
+    step = Step([(1, 3), (1, 0), (20, 13)], page, gen)
+    pages = random_pages(step.pages, Hkv, D, page, gen)
+    plain = PlainPages.of(pages)
+    rows, rows64 = _rows(step.T, Hq, Hkv, D, gen, gap=offset, offset=offset, values_are_keys=same)
+    qw, kw = (1 + 0.2 * torch.randn(D, generator=gen), 1 + 0.2 * torch.randn(D, generator=gen)) if norm else (None, None)
+    table = rotation(64, D) if turn else None
+    on = lambda t: None if t is None else t.to(DEV)  # noqa: E731
+    q = ops.qk_norm_rope_store_e4m3(rows, on(qw), on(kw), EPS, on(table), step.positions.to(DEV), step.slots.to(DEV), pages, Hq, Hkv, D, page,
+                                    values_are_keys=same)
+    eq, ek, ev = _append_plain(rows64, step, plain, Hq, Hkv, D, qw, kw, table, same)
+    _check_append(rows, q, pages, plain, None, step, ek, ev, eq)
+
+
+def test_append_token_by_token():
+    """One token after another, growing and not: every step's bytes are the plain form's (no norm, no rotation: nothing is computed)."""
+    Hkv, D, page = 3, 48, 16
+    gen = _gen(11)
+    pages = empty_pages(3, Hkv, D, page)
+    plain = PlainPages.of(pages)
+    for t in range(40):
+        x = torch.randn(1, 2 * Hkv * D, generator=gen) * 10.0 ** float(torch.randint(-3, 4, (1,), generator=gen))
+        x = x.to(torch.bfloat16)
+        slot = torch.tensor([16 + t if t < 32 else t - 32], dtype=torch.int32)
+        ops.qk_norm_rope_store_e4m3(x.to(DEV), None, None, EPS, None, slot.to(DEV), slot.to(DEV), pages, 0, Hkv, D, page)
+        h = x.double().view(1, 2 * Hkv, D)
+        plain.place(h[:, :Hkv], h[:, Hkv:], [int(slot)])
+        got = PlainPages.of(pages)
+        assert torch.equal(got.k, plain.k) and torch.equal(got.v, plain.v) and torch.equal(got.kp, plain.kp) and torch.equal(got.vp, plain.vp), t
+
+
+def test_append_of_nothing_computed_is_the_plain_forms_bytes():
+    """Every bfloat16 number of ordinary size, as keys and values; a second identical call changes nothing."""
+    Hkv, D, page = 2, 64, 16
+    x = torch.arange(1 << 16, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    x = x[torch.isfinite(x.float()) & (x.float().abs() < 3e4)]
+    T = x.numel() // (2 * Hkv * D)
+    x = x[torch.randperm(x.numel(), generator=_gen(0))][:T * 2 * Hkv * D].view(T, -1)
+    pages = empty_pages(-(-T // page) + 1, Hkv, D, page)
+    slots = torch.arange(T, dtype=torch.int32) + page
+    plain = PlainPages.of(pages)
+    h = x.double().view(T, 2 * Hkv, D)
+    plain.place(h[:, :Hkv], h[:, Hkv:], slots.tolist())
+    for _ in range(2):
+        ops.qk_norm_rope_store_e4m3(x.to(DEV), None, None, EPS, None, slots.to(DEV), slots.to(DEV), pages, 0, Hkv, D, page)
+        got = PlainPages.of(pages)
+        assert torch.equal(got.k, plain.k) and torch.equal(got.v, plain.v) and torch.equal(got.kp, plain.kp) and torch.equal(got.vp, plain.vp)
+
+
+@pytest.mark.parametrize("slots", [[16] * 40, [16, 17, 18, 17, 18, 19], [20, 19, 18], [3, 3, 3, 0, 1, 1], list(range(16, 32)) * 5 + [16, 17],
+                                   [31, 16, 5, -1, 6, -7, 5, 1000, 7], [17] * 100 + [18] * 3, [0] * 300, list(range(16)) * 20])
+def test_append_rows_out_of_order(slots):
+    """Rows of a block that follow each other out of order are calls one after the other; what a later one opens anew is forgotten.
+    Slots that name no place are skipped (1000 lies behind the last page)."""
+    Hkv, D, page = 2, 32, 16
+    gen = _gen(len(slots))
+    pages = random_pages(3, Hkv, D, page, gen)
+    plain = PlainPages.of(pages)
+    x = (torch.randn(len(slots), 2 * Hkv * D, generator=gen) * torch.exp(2 * torch.randn(len(slots), 1, generator=gen))).to(torch.bfloat16)
+    s = torch.tensor(slots, dtype=torch.int32)
+    ops.qk_norm_rope_store_e4m3(x.to(DEV), None, None, EPS, None, s.to(DEV), s.to(DEV), pages, 0, Hkv, D, page)
+    h = x.double().view(len(slots), 2 * Hkv, D)
+    # rows [start, end) of one block; the next ones of the same block that begin at its place 0 make them forgotten
+    valid = [v if 0 <= v < 3 * page else -1 for v in slots]
+    goes_on = lambda t: t > 0 and valid[t] >= 0 and valid[t - 1] >= 0 and valid[t] // BLOCK == valid[t - 1] // BLOCK  # noqa: E731
+    starts = [t for t in range(len(valid)) if not goes_on(t) or valid[t] % BLOCK == 0] + [len(valid)]
+    kept = []
+    for t, e in zip(starts, starts[1:]):
+        if valid[t] >= 0 and not (e < len(valid) and goes_on(e)):
+            kept += range(t, e)
+    keep = torch.tensor(kept)
+    plain.place(h[keep, :Hkv], h[keep, Hkv:], [slots[t] for t in kept])
+    got = PlainPages.of(pages)
+    # a block whose rows stand apart (others or skipped ones between them) is in no order: any of them may be its last
+    apart = [valid[t] // BLOCK for t in range(len(valid)) if valid[t] >= 0 and not goes_on(t)]
+    sure = [b for b in range(3) if apart.count(b) <= 1]
+    for x, y in ((got.kp, plain.kp), (got.vp, plain.vp), (got.k, plain.k), (got.v, plain.v)):
+        assert torch.equal(x[sure], y[sure])
+
+
+def test_append_numbers_that_are_none():
+    """Infinities and NaN are stored as NaN and leave the block's power to the others."""
+    Hkv, D, page = 1, 32, 16
+    x = torch.randn(4, 2 * D, generator=_gen(1)).to(torch.bfloat16)
+    x[0, 3] = math.inf
+    x[1, 5] = -math.inf
+    x[2, D + 1] = math.nan
+    x[3] = math.nan
+    pages = empty_pages(2, Hkv, D, page)
+    plain = PlainPages.of(pages)
+    slots = torch.tensor([16, 17, 18, 0], dtype=torch.int32)
+    ops.qk_norm_rope_store_e4m3(x.to(DEV), None, None, EPS, None, slots.to(DEV), slots.to(DEV), pages, 0, Hkv, D, page)
+    h = x.double().view(4, 2, D)
+    plain.place(h[:, :1], h[:, 1:], slots.tolist())
+    got = PlainPages.of(pages)
+    assert torch.equal(got.kp, plain.kp) and torch.equal(got.vp, plain.vp) and got.kp[0, 0, 0] == LEAST
+    assert torch.equal(torch.isnan(got.k), torch.isnan(plain.k)) and torch.equal(got.k.nan_to_num(), plain.k.nan_to_num())
+    assert torch.equal(torch.isnan(got.v), torch.isnan(plain.v)) and torch.equal(got.v.nan_to_num(), plain.v.nan_to_num())
+
+
+def test_append_no_rows():
+    pages = empty_pages(2, 2, 32, 16)
+    none = torch.zeros(0, dtype=torch.int32, device=DEV)
+    q = ops.qk_norm_rope_store_e4m3(torch.zeros(0, 8 * 32, dtype=torch.bfloat16, device=DEV), None, None, EPS, None, none, none, pages, 4, 2, 32, 16)
+    assert q.shape == (0, 128)
+
+
+# ------------------------------------------------------------------ attention
+
+def _attention(q, pages, step, scale, Hq, Hkv, D, window=None, chunk=None, sinks=None):
+    on = lambda t: None if t is None else t.to(DEV)  # noqa: E731
+    return ops.paged_attention_e4m3(q, pages, step.page, on(step.tables), on(step.contexts), on(step.seq), on(step.positions), on(step.cu), step.decode,
+                                    step.decode_context, scale, window, Hq, Hkv, D, max_prefill_context=step.prefill_context, chunk=chunk, sinks=on(sinks))
+
+
+def _check_attention(lengths, Hq, Hkv, D, page, seed=0, gap=0, pages=None, loud=1.0, **options):
+    gen = _gen(seed)
+    step = Step(lengths, page, gen)
+    pages = mild_pages(step.pages, Hkv, D, page, gen) if pages is None else pages(step, gen)
+    q = (loud * torch.randn(step.T, Hq * D + gap, generator=gen)).to(torch.bfloat16)
+    scale = D ** -0.5
+    got = _attention(q.to(DEV)[:, :Hq * D], pages, step, scale, Hq, Hkv, D, **options)
+    o, spread = attend(q[:, :Hq * D].double().view(step.T, Hq, D), PlainPages.of(pages).numbers(), step, scale, Hq, Hkv, **options)
+    got = got.cpu().double().view(step.T, Hq, D)
+    assert torch.equal(torch.isnan(got), torch.isnan(o))
+    off = (got - o).abs() - attention_bound(o, spread)
+    assert (off.nan_to_num() <= 0).all(), float(off.nan_to_num().max())
+    return got, o, step
+
+
+MIX = [(1, 0), (1, 1), (1, 62), (1, 63), (1, 64), (1, -1), (1, 300), (1, 255), (2, 0), (65, 0), (7, 130), (129, 16)]
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", HEADS + [(20, 1, 32), (40, 2, 128), (12, 1, 96)])
+@pytest.mark.parametrize("page", [16, 128])
+def test_attention_mixed_step(Hq, Hkv, D, page):
+    """Contexts of one key to several blocks, a padding row, portions of all kinds."""
+    _check_attention(MIX, Hq, Hkv, D, page, seed=D, gap=8)
+
+
+@pytest.mark.parametrize("options", [dict(window=1), dict(window=16), dict(window=63), dict(window=100), dict(chunk=8), dict(chunk=50), dict(window=40, sinks=True),
+                                     dict(sinks=True), dict(chunk=64, sinks=True)])
+@pytest.mark.parametrize("Hq,Hkv,D", [(4, 2, 64), (8, 8, 32)])
+def test_attention_masks(options, Hq, Hkv, D):
+    if options.get("sinks"):
+        options = dict(options, sinks=torch.randn(Hq, generator=_gen(5)))
+    _check_attention(MIX, Hq, Hkv, D, 16, seed=1, **options)
+
+
+@pytest.mark.parametrize("lengths", [[(1, 9999)], [(1, 40000), (1, 3)], [(1, 2047)] * 8, [(300, 5000)], [(2, 9000)], [(700, 0), (500, 300)], [(1, 700)] * 70])
+@pytest.mark.parametrize("window", [None, 1000])
+def test_attention_long(lengths, window):
+    """Ranges that are cut into partitions and joined."""
+    _check_attention(lengths, 8, 2, 128, 32, seed=2, window=window)
+
+
+def test_attention_uneven_scores():
+    """Loud queries: a few keys have all of the softmax, and the maximum rises again and again."""
+    got, o, _ = _check_attention(MIX + [(200, 900)], 4, 2, 64, 16, seed=3, loud=20.0)
+
+
+def test_attention_nan_where_nobody_looks():
+    """Foreign and unwritten places hold NaN, in pages of others, behind the context and in front of the window: no row may notice. A key or a
+    value that is NaN makes NaN of the rows (the value: of its channel in the rows) that see it, and of no other."""
+    def pages(step, gen):
+        p = mild_pages(step.pages, 2, 32, 16, gen)
+        k, v = p.k.view(torch.uint8), p.v.view(torch.uint8)
+        held = {}
+        for table, L in zip(step.table_rows, step.contexts.tolist()):
+            for i, pg in enumerate(table):
+                held[pg] = (i * 16, L)
+        for pg in range(step.pages):
+            first, L = held.get(pg, (0, 0))
+            for off in range(16):
+                if first + off >= L or first + off < 3:       # behind the end; in front of what a window of 40 shows the last rows
+                    if first + off >= L or L > 60:
+                        k[pg, :, off] = 0x7F
+                        v[pg, :, :, off] = 0xFF
+        return p
+    _check_attention([(1, 99), (1, 0), (1, 64), (3, 110), (20, 61)], 4, 2, 32, 16, seed=4, pages=pages, window=40)
+
+    def one_value(step, gen):
+        p = mild_pages(step.pages, 2, 32, 16, gen)
+        pg = step.table_rows[0][50 // 16]
+        p.v.view(torch.uint8)[pg, 1, 7, 50 % 16] = 0x7F
+        return p
+    got, o, step = _check_attention([(90, 0)], 4, 2, 32, 16, seed=5, pages=one_value)
+    assert torch.isnan(got[50:, 2:, 7]).all() and not torch.isnan(got[:50]).any() and int(torch.isnan(got).sum()) == 40 * 2
+
+    def one_key(step, gen):
+        p = mild_pages(step.pages, 2, 32, 16, gen)
+        p.k.view(torch.uint8)[step.table_rows[0][50 // 16], 1, 50 % 16, 7] = 0xFF
+        return p
+    gen = _gen(6)
+    step = Step([(90, 0)], 16, gen)
+    p = one_key(step, gen)
+    q = torch.randn(step.T, 128, generator=gen).to(torch.bfloat16).to(DEV)
+    got = _attention(q, p, step, 0.2, 4, 2, 32)
+    assert torch.isnan(got[50:, 64:].float()).all() and not torch.isnan(got[:50].float()).any() and not torch.isnan(got[:, :64].float()).any()
+
+
+def test_attention_tables_with_holes():
+    """Keys of table entries that hold no page, or name none, are not seen; a row that sees nothing gets zeros."""
+    gen = _gen(8)
+    step = Step([(1, 100), (1, 20), (30, 40)], 16, gen)
+    pages = mild_pages(step.pages, 2, 64, 16, gen)
+    for r, i, bad in ((0, 2, -1), (0, 3, 1 << 30), (1, 0, -1), (1, 1, -5), (2, 0, step.pages)):
+        step.table_rows[r][i] = -1
+        step.tables[r, i] = bad
+    q = torch.randn(step.T, 4 * 64, generator=gen).to(torch.bfloat16)
+    got = _attention(q.to(DEV), pages, step, 0.1, 4, 2, 64).cpu().double().view(step.T, 4, 64)
+    o, spread = attend(q.double().view(step.T, 4, 64), PlainPages.of(pages).numbers(), step, 0.1, 4, 2)
+    assert ((got - o).abs() <= attention_bound(o, spread)).all() and not got[1].any()
+
+
+def test_attention_of_no_rows():
+    pages = mild_pages(2, 2, 32, 16, _gen(0))
+    z = torch.zeros(0, dtype=torch.int32, device=DEV)
+    out = ops.paged_attention_e4m3(torch.zeros(0, 128, dtype=torch.bfloat16, device=DEV), pages, 16, torch.zeros(0, 1, dtype=torch.int32, device=DEV), z, z, z,
+                                   None, 0, 0, 1.0, None, 4, 2, 32)
+    assert out.shape == (0, 128)
+
+
+def test_the_same_call_gives_the_same_bits():
+    gen = _gen(9)
+    step = Step([(1, 5000), (1, 100), (300, 2000)], 32, gen)
+    pages = mild_pages(step.pages, 2, 128, 32, gen)
+    q = torch.randn(step.T, 8 * 128, generator=gen).to(torch.bfloat16).to(DEV)
+    first = _attention(q, pages, step, 0.1, 8, 2, 128)
+    for _ in range(3):
+        assert torch.equal(first, _attention(q, pages, step, 0.1, 8, 2, 128))
+
+
+def test_a_step_after_another():
+    """A prompt in portions and then token by token, appended and attended to through the cache alone: every row against 64 bits."""
+    Hq, Hkv, D, page = 8, 2, 64, 16
+    gen = _gen(10)
+    pages, table = empty_pages(20, Hkv, D, page), rotation(256, D)
+    plain = PlainPages.of(pages)
+    order = torch.randperm(20, generator=gen).tolist()
+    w = torch.ones(D)
+    kept = 0
+    for n in (50, 1, 1, 37, 1, 70, 1, 1, 1):
+        step = Step([(n, kept)], page, gen)
+        step.table_rows = [order[:-(-(n + kept) // page)]]
+        step.tables = torch.tensor(step.table_rows, dtype=torch.int32)
+        step.slots = torch.tensor([order[p // page] * page + p % page for p in range(kept, kept + n)], dtype=torch.int32)
+        rows, rows64 = _rows(n, Hq, Hkv, D, gen)
+        q = ops.qk_norm_rope_store_e4m3(rows, w.to(DEV), w.to(DEV), EPS, table.to(DEV), step.positions.to(DEV), step.slots.to(DEV), pages, Hq, Hkv, D, page)
+        got = _attention(q, pages, step, D ** -0.5, Hq, Hkv, D).cpu().double().view(n, Hq, D)
+        eq, ek, ev = _append_plain(rows64, step, plain, Hq, Hkv, D, w, w, table)
+        _check_append(rows, q, pages, plain, None, step, ek, ev, eq, values_exact=True)
+        o, spread = attend(q.cpu().double().view(n, Hq, D), PlainPages.of(pages).numbers(), step, D ** -0.5, Hq, Hkv)
+        assert ((got - o).abs() <= attention_bound(o, spread)).all()
+        plain.k = PlainPages.of(pages).k            # the few keys at a rounding's border, as they fell
+        kept += n
+
+
+def test_captured_step_is_replayed():
+    """Append and attention in a graph, replayed with other inputs, eager work between the replays; the caches' bytes too."""
+    Hq, Hkv, D, page = 8, 2, 128, 16
+    gen = _gen(12)
+    step = Step([(1, 900), (1, 30), (1, -1), (60, 20)], page, gen)
+    pages, other = (mild_pages(step.pages, Hkv, D, page, _gen(13)) for _ in range(2))
+    table, w = rotation(1024, D).to(DEV), torch.ones(D, device=DEV)
+    rows = torch.zeros(step.T, (Hq + 2 * Hkv) * D, dtype=torch.bfloat16, device=DEV)
+    on = {n: getattr(step, n).to(DEV) for n in ("tables", "contexts", "seq", "positions", "cu", "slots")}
+
+    def run(rows, pages):
+        q = ops.qk_norm_rope_store_e4m3(rows, w, w, EPS, table, on["positions"], on["slots"], pages, Hq, Hkv, D, page)
+        return ops.paged_attention_e4m3(q, pages, page, on["tables"], on["contexts"], on["seq"], on["positions"], on["cu"], step.decode, step.decode_context,
+                                        D ** -0.5, None, Hq, Hkv, D, max_prefill_context=step.prefill_context)
+    run(rows, pages)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(rows, pages)
+    for p, o in zip(pages.tensors(), other.tensors()):
+        p.copy_(o) if p.dtype == torch.uint8 else p.view(torch.uint8).copy_(o.view(torch.uint8))
+    for seed in range(4):
+        x = torch.randn(rows.shape, generator=_gen(seed)).to(torch.bfloat16)
+        rows.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = run(x.to(DEV), other)
+        torch.cuda.synchronize()
+        live = torch.tensor([i for i in range(step.T) if i != 2], device=DEV)
+        assert torch.equal(out[live], eager[live]) and not out[2].any()
+        for p, o in zip(pages.tensors(), other.tensors()):
+            assert torch.equal(p.view(torch.uint8), o.view(torch.uint8))
+
+
+def test_calls_on_two_streams_do_not_meet():
+    """Two launches side by side, both cut into partitions, on streams of their own."""
+    gen = _gen(14)
+    step = Step([(1, 6000), (200, 3000)], 32, gen)
+    pages = mild_pages(step.pages, 2, 128, 32, gen)
+    qs = [torch.randn(step.T, 8 * 128, generator=gen).to(torch.bfloat16).to(DEV) for _ in range(2)]
+    expect = [_attention(q, pages, step, 0.1, 8, 2, 128) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    on = {n: getattr(step, n).to(DEV) for n in ("tables", "contexts", "seq", "positions", "cu")}
+    torch.cuda.synchronize()
+    for _ in range(5):
+        found = []
+        for q, s in zip(qs, streams):
+            with torch.cuda.stream(s):
+                found.append(ops.paged_attention_e4m3(q, pages, 32, on["tables"], on["contexts"], on["seq"], on["positions"], on["cu"], step.decode,
+                                                      step.decode_context, 0.1, None, 8, 2, 128, max_prefill_context=step.prefill_context))
+        torch.cuda.synchronize()
+        for a, b in zip(found, expect):
+            assert torch.equal(a, b)
+
+
+def test_tensors_elsewhere_are_refused():
+    gen = _gen(15)
+    step = Step([(1, 20)], 16, gen)
+    pages = mild_pages(step.pages, 2, 32, 16, gen)
+    q = torch.randn(1, 128, generator=gen).to(torch.bfloat16)
+    with pytest.raises(ops.KernelError, match="current GPU"):
+        _attention(q, pages, step, 0.1, 4, 2, 32)
+    with pytest.raises(ops.KernelError, match="current GPU"):
+        ops.qk_norm_rope_store_e4m3(torch.zeros(1, 8 * 32, dtype=torch.bfloat16, device=DEV), None, None, EPS, None, step.positions, step.slots.to(DEV), pages, 4,
+                                    2, 32, 16)
+    with pytest.raises(ops.KernelError, match="beyond the rotation table"):
+        ops.qk_norm_rope_store_e4m3(torch.zeros(1, 8 * 32, dtype=torch.bfloat16, device=DEV), None, None, EPS, rotation(8, 32).to(DEV), step.positions.to(DEV),
+                                    step.slots.to(DEV), pages, 4, 2, 32, 16, position_bound=21)
