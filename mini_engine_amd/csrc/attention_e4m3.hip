@@ -18,7 +18,7 @@
 // Keys that a column does not see are replaced, never multiplied by zero: scores by "none", stored values by zero bytes where no
 // column sees them, and where some columns of a tile see a key whose value is NaN and others do not, only those that see it become NaN.
 #include "e4m3.h"
-#include <cstdlib>
+#include <type_traits>
 
 #ifndef ME_HEAD_DIM
 #error "compile with -DME_HEAD_DIM=<multiple of 16>"
@@ -160,125 +160,104 @@ __device__ __forceinline__ void hide_values(Block& b, int t0, int lo, int L, int
 
 template <int CT>
 struct Columns {
-  bf16x8 q[CT][2 * KL];
   int lo[CT], hi[CT];            // keys [lo, hi] that the column sees (hi < lo: none)
   float m[CT], l[CT];            // reference point of the exponentials (log2 domain), this lane's share of the sum
   f32x4 acc[CT][DT];
 };
 
-// One block for all columns of a wave. FULL: every column sees every key of it, and all of them lie in pages.
-template <int CT, bool FULL>
-__device__ __forceinline__ void attend(const Attn8Args& a, Block& b, int t0, int lo, int L, int g, Columns<CT>& c) {
+// The softmax of N tiles of scores (4 N keys of a lane, from `first` on) in column tile ct: under the column's reference point, which
+// rises where it must (the column's sums with it), their probabilities are added to the sum and rounded to bfloat16 as the second
+// product's operand (the sum takes them unrounded). FULL: the column sees all keys; else `seen` gets the bits of the lane's keys that
+// it does. there: they lie in a page.
+template <int CT, bool FULL, int N>
+__device__ __forceinline__ void softmax_tiles(const f32x4* st, float sc, int first, bool there, int ct, Columns<CT>& c, uint32_t& seen, bf16x8* pb) {
+  float s[4 * N];
+  float top = NONE;
+  if constexpr (!FULL) {
+    const int from = max(c.lo[ct] - first, 0), to = min(c.hi[ct] - first, 4 * N - 1);
+    seen = there && to >= from && from < 4 * N ? (2u << to) - (1u << from) : 0u;
+  }
+#pragma unroll
+  for (int i = 0; i < 4 * N; ++i) {
+    s[i] = st[i >> 2][i & 3];
+    if constexpr (!FULL) s[i] = (seen >> i) & 1 ? s[i] : NONE;
+    top = fmaxf(top, s[i]);
+  }
+  if (__any(top > 0.5f * NONE && top * sc > c.m[ct] + RESCALE_STEP)) {
+    top = max_of_column(top);
+    const float next = top > 0.5f * NONE ? top * sc : NONE;
+    if (next > c.m[ct] + RESCALE_STEP) {
+      const float f = __builtin_amdgcn_exp2f(c.m[ct] - next);
+      c.l[ct] *= f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c.acc[ct][dt][i] *= f;
+      c.m[ct] = next;
+    }
+  }
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4 * N; ++i) {
+    float p = __builtin_amdgcn_exp2f(fmaf(s[i], sc, -c.m[ct]));
+    if constexpr (!FULL) p = (seen >> i) & 1 ? p : 0.f;      // while a column has seen no key, its reference point is NONE too
+    sum += p;
+    pb[i >> 3][i & 7] = static_cast<bf16_t>(p);
+  }
+  c.l[ct] += sum;
+}
+
+// The second product of one channel tile where a value may be NaN that some columns see and others do not: NaN counts as zero, and
+// whoever sees one becomes NaN (a product of what is NaN and what is seen counts them).
+template <int CT>
+__device__ __forceinline__ void values_with_nan(bf16x8 va, const uint32_t (&seen)[CT], const bf16x8 (&pb)[CT], int dt, Columns<CT>& c) {
+  bf16x8 bad;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const bool is = static_cast<float>(va[e]) != static_cast<float>(va[e]);
+    bad[e] = static_cast<bf16_t>(is ? 1.f : 0.f);
+    va[e] = is ? static_cast<bf16_t>(0.f) : va[e];
+  }
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    bf16x8 sees;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sees[e] = static_cast<bf16_t>((seen[ct] >> e) & 1 ? 1.f : 0.f);
+    const f32x4 count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bad, sees, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+    c.acc[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pb[ct], c.acc[ct][dt], 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c.acc[ct][dt][i] = count[i] > 0.f ? __uint_as_float(0x7fc00000u) : c.acc[ct][dt][i];
+  }
+}
+
+// One block out of registers, for a wave's single column tile. FULL: every column sees every key of it, and all of them lie in pages.
+// (Otherwise all columns see the same keys: what none of them sees is zeroed, and a NaN among the others is everybody's.)
+template <bool FULL>
+__device__ __forceinline__ void attend(const Attn8Args& a, Block& b, int t0, int lo, int L, int g, const bf16x8 (&q)[2 * KL], Columns<1>& c) {
   const float kpow = power_of(b.kcode), vpow = power_of(b.vcode);
-  const float sc = a.scale * LOG2E;
-  f32x4 st[CT][4];
+  f32x4 st[4];
 #pragma unroll
   for (int tt = 0; tt < 4; ++tt) {
-    bf16x8 ka[2 * KL];
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < KL; ++j) {
       const bool in = HD % 64 == 0 || 64 * j + 16 * g < HD;
       u32x4v w = b.k[tt][j];
       if (!in) w = u32x4v{0, 0, 0, 0};
-      ka[2 * j] = operand(w[0], w[1], kpow);
-      ka[2 * j + 1] = operand(w[2], w[3], kpow);
+      s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(w[0], w[1], kpow), q[2 * j], s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(w[2], w[3], kpow), q[2 * j + 1], s, 0, 0, 0);
     }
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      f32x4 s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int ks = 0; ks < 2 * KL; ++ks) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka[ks], c.q[ct][ks], s, 0, 0, 0);
-      st[ct][tt] = s;
-    }
+    st[tt] = s;
   }
-  bf16x8 pb[CT][2];
-  uint32_t seen[CT];             // bit i: the column sees this lane's key i
+  bf16x8 pb[2];
+  uint32_t seen;
+  softmax_tiles<1, FULL, 4>(st, a.scale * LOG2E, t0 + 16 * g, b.there, 0, c, seen, pb);
+  if constexpr (!FULL) hide_values(b, t0, lo, L, g);
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    float s[16];
-    float top = NONE;
-    seen[ct] = 0xffffu;
-    if constexpr (!FULL) {
-      const int from = max(c.lo[ct] - (t0 + 16 * g), 0), to = min(c.hi[ct] - (t0 + 16 * g), 15);
-      seen[ct] = b.there && to >= from && from < 16 ? (2u << to) - (1u << from) : 0u;
-    }
+  for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s[i] = st[ct][i >> 2][i & 3];
-      if constexpr (!FULL) s[i] = (seen[ct] >> i) & 1 ? s[i] : NONE;
-      top = fmaxf(top, s[i]);
-    }
-    if (__any(top > 0.5f * NONE && top * sc > c.m[ct] + RESCALE_STEP)) {
-      top = max_of_column(top);
-      const float next = top > 0.5f * NONE ? top * sc : NONE;
-      if (next > c.m[ct] + RESCALE_STEP) {
-        const float f = __builtin_amdgcn_exp2f(c.m[ct] - next);
-        c.l[ct] *= f;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) c.acc[ct][dt][i] *= f;
-        c.m[ct] = next;
-      }
-    }
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float p = __builtin_amdgcn_exp2f(fmaf(s[i], sc, -c.m[ct]));
-      if constexpr (!FULL) p = (seen[ct] >> i) & 1 ? p : 0.f;
-      sum += p;
-      pb[ct][i >> 3][i & 7] = static_cast<bf16_t>(p);      // the sum takes it unrounded
-    }
-    c.l[ct] += sum;
-  }
-  if constexpr (!FULL) {
-    hide_values(b, t0, lo, L, g);
-    uint32_t any = 0;            // a stored NaN: all seven lower bits of a byte
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-      for (int w = 0; w < 4; ++w) any |= (b.v[dt][w] & 0x7f7f7f7fu) + 0x01010101u;
-    if (__any((any & 0x80808080u) != 0)) {
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        bf16x8 va[2], bad[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          va[h] = operand(b.v[dt][2 * h], b.v[dt][2 * h + 1], vpow);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const bool is = ((b.v[dt][2 * h + (e >> 2)] >> (8 * (e & 3))) & 0x7f) == 0x7f;
-            bad[h][e] = static_cast<bf16_t>(is ? 1.f : 0.f);
-            va[h][e] = is ? static_cast<bf16_t>(0.f) : va[h][e];
-          }
-        }
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          f32x4 count = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            bf16x8 sees;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sees[e] = static_cast<bf16_t>((seen[ct] >> (8 * h + e)) & 1 ? 1.f : 0.f);
-            count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bad[h], sees, count, 0, 0, 0);
-            c.acc[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va[h], pb[ct][h], c.acc[ct][dt], 0, 0, 0);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) c.acc[ct][dt][i] = count[i] > 0.f ? __uint_as_float(0x7fc00000u) : c.acc[ct][dt][i];
-        }
-      }
-      return;
-    }
-  }
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const bf16x8 va = operand(b.v[dt][2 * h], b.v[dt][2 * h + 1], vpow);
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) c.acc[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pb[ct][h], c.acc[ct][dt], 0, 0, 0);
-    }
-  }
+    for (int h = 0; h < 2; ++h)
+      c.acc[0][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(b.v[dt][2 * h], b.v[dt][2 * h + 1], vpow), pb[h], c.acc[0][dt], 0, 0, 0);
 }
 
 // A softmax's denominator with its head's sink; a column that saw no key stays at zero.
@@ -313,14 +292,16 @@ __global__ void __launch_bounds__(256) attn8_decode_kernel(Attn8Args a) {
   for (int dt = 0; dt < DT; ++dt) c.acc[0][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   int t0 = p_lo + BK * wave;
   if (t0 < p_hi) {
-    load_q(a.q + b * a.q_stride + (int64_t)head * HD, valid, g, c.q[0]);
+    bf16x8 q[2 * KL];
+    load_q(a.q + b * a.q_stride + (int64_t)head * HD, valid, g, q);
+
     Block blk;
     load_block(a, find_pages(a, table, t0, lo, L, n, g), kvh, t0, lo, L, n, g, blk);
     while (true) {
       // a block whose pages are all there and whose keys the token sees: whole-wave test
       const bool full = t0 >= lo && t0 + BK <= p_hi && __all(blk.there);
-      if (full) attend<1, true>(a, blk, t0, lo, L, g, c);
-      else attend<1, false>(a, blk, t0, lo, L, g, c);
+      if (full) attend<true>(a, blk, t0, lo, L, g, q, c);
+      else attend<false>(a, blk, t0, lo, L, g, q, c);
       t0 += 4 * BK;
       if (t0 >= p_hi) break;
       load_block(a, find_pages(a, table, t0, lo, L, n, g), kvh, t0, lo, L, n, g, blk);
@@ -361,11 +342,33 @@ __global__ void __launch_bounds__(256) attn8_decode_kernel(Attn8Args a) {
 }
 
 // =====================================================================================
-// Portions of prompts. A tile is 64 CT columns of one request and key head; each of the 4 waves of its workgroup has 16 CT of
-// them and walks the keys that they see. Grid (tiles x key heads, segments): surplus tiles (the grid is made for the most there can be) exit.
+// Portions of prompts. A tile is 64 CT columns of one request and key head; each of the 4 waves of its workgroup has 16 CT of them.
+// The workgroup walks the keys that its columns see in blocks of 32 (key 8 (m / 4) + 4 tt + m % 4 in row m of tile tt: lane (n, g) ends
+// with the 8 keys from 8 g on). A block's bytes are read once, three blocks ahead, and turned into bfloat16 once, two blocks ahead, in LDS,
+// from which every wave reads its operands (each wave all conversions for itself would be a third of its vector instructions). What a wave
+// reads of a block lies in one page under one power, so pages and addresses are scalars.
+//   keys    [32][KROW]: row 16 tt + m, channels in order, and 16 bytes of padding, so that the 16 rows of a read lie in 16 different
+//           groups of banks. Channels from HD to the next 32 are zero.
+//   values  [HD][VROW]: 32 keys and the same padding.
+// Step k of the walk is a pipeline: beside the numbers of block k's softmax the products of block k + 1's scores, beside the products of
+// its values block k + 2's conversion. Three LDS buffers, one barrier a step.
+// Grid (tiles x key heads, segments): surplus tiles (the grid is made for the most there can be) exit.
 // =====================================================================================
+constexpr int PB = 32;                       // keys of a block
+constexpr int KS = (HD + 31) / 32;           // products of a tile of scores
+constexpr int KROW = 64 * KS + 16, VROW = 2 * PB + 16;                     // bytes
+constexpr int VBASE = PB * KROW, BUF = VBASE + HD * VROW;
+constexpr int PIECES = (HD + 127) / 128;     // 16-byte pieces of keys (and of values) of a block that a lane brings
+
+struct Staged {
+  u32x4v k[PIECES], v[PIECES];
+  uint32_t kcode, vcode;
+};
+
 template <int CT>
-__global__ void __launch_bounds__(256) attn8_prompt_kernel(Attn8Args a, int tiles) {
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 128 ? 2 : 1, HD <= 128 ? 2 : 1))) attn8_prompt_kernel(Attn8Args a, int tiles) {
+  extern __shared__ __align__(16) char lds_bytes[];        // three buffers, then a flag for each of four blocks in a row
+  int* flags = reinterpret_cast<int*>(lds_bytes + 3 * BUF);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
   const int kvh = blockIdx.x % a.Hkv, tile = tiles - 1 - (int)(blockIdx.x / a.Hkv), seg = blockIdx.y;
@@ -380,64 +383,287 @@ __global__ void __launch_bounds__(256) attn8_prompt_kernel(Attn8Args a, int tile
   const int col0 = (tile - (int)((int64_t)q0 * a.G / COLS) - b) * COLS;
   if (col0 >= q_len * a.G) return;
   const int L = context_of(a, b), start = L - q_len;
-  const int32_t* table = a.tables + (int64_t)b * a.table_stride;
+  const int32_t* __restrict__ table = a.tables + (int64_t)b * a.table_stride;
   // the keys that the tile's columns see, and this segment's share of them
   const int last_tok = min(col0 + COLS, q_len * a.G) - 1;
   const int tile_lo = first_seen(a, max(start + col0 / a.G, 0)), tile_hi = start + last_tok / a.G + 1;
-  const int base = tile_lo & ~(BK - 1);
-  const int seg_lo = base + seg * a.part_keys, seg_hi = seg + 1 < a.num_parts ? min(tile_hi, seg_lo + a.part_keys) : tile_hi;
+  const int seg_lo = (tile_lo & ~(BK - 1)) + seg * a.part_keys, seg_hi = seg + 1 < a.num_parts ? min(tile_hi, seg_lo + a.part_keys) : tile_hi;
+  const int nblk = (seg_hi - seg_lo + PB - 1) / PB;           // (none: not above 0)
+
+  bf16x8 q[CT][KS];
   Columns<CT> c;
-  int64_t row[CT];
-  int head[CT];
-  bool valid[CT];
-  int wave_lo = 0x7fffffff, wave_hi = 0, all_lo = 0, all_hi = 0x7fffffff;
+  int all_lo = 0, all_hi = 0x7fffffff;
+  bool whole = true;
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     const int col = col0 + (wave * CT + ct) * 16 + n;
-    valid[ct] = col < q_len * a.G;
-    const int tok = valid[ct] ? col / a.G : 0;
-    head[ct] = kvh * a.G + (valid[ct] ? col - tok * a.G : 0);
-    row[ct] = q0 + tok;
+    const bool valid = col < q_len * a.G;
+    const int tok = valid ? col / a.G : 0;
+    const int head = kvh * a.G + (valid ? col - tok * a.G : 0);
     c.m[ct] = NONE; c.l[ct] = 0.f;
-    c.hi[ct] = valid[ct] ? start + tok : -1;
-    c.lo[ct] = valid[ct] ? first_seen(a, max(start + tok, 0)) : 0;
-    load_q(a.q + row[ct] * a.q_stride + (int64_t)head[ct] * HD, valid[ct], g, c.q[ct]);
+    c.hi[ct] = valid ? start + tok : -1;
+    c.lo[ct] = valid ? first_seen(a, max(start + tok, 0)) : 0;
+    const bf16_t* row = a.q + (q0 + tok) * a.q_stride + (int64_t)head * HD;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const bool in = HD % 32 == 0 || 32 * ks + 8 * g < HD;
+      bf16x8 x = *reinterpret_cast<const bf16x8*>(row + (in ? 32 * ks + 8 * g : 0));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = valid && in ? x[e] : static_cast<bf16_t>(0.f);
+      q[ct][ks] = x;
+    }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) c.acc[ct][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (valid[ct]) {
-      wave_lo = min(wave_lo, c.lo[ct]); wave_hi = max(wave_hi, c.hi[ct] + 1);
-      all_lo = max(all_lo, c.lo[ct]); all_hi = min(all_hi, c.hi[ct]);
+    whole = whole && valid;
+    all_lo = max(all_lo, c.lo[ct]); all_hi = min(all_hi, c.hi[ct]);
+  }
+  // (a wave's columns are in order: the first one that does not see a key is the last or the first of them)
+  all_lo = __builtin_amdgcn_readlane(all_lo, 15); all_hi = __builtin_amdgcn_readlane(all_hi, 0);
+  if (!__all(whole)) all_hi = -1;
+
+  if (nblk > 0) {
+    const int group = wave >> 1, part = wave & 1;             // this wave brings half of a block's 16 keys `group`: 8 keys, HD / 2 channels of values
+    const int page_mask = (1 << a.page_shift) - 1;
+    if (HD % 32 != 0 && threadIdx.x < 3 * PB) {               // the channels that no head has: zeros, once
+      char* pad = lds_bytes + (threadIdx.x / PB) * BUF + (threadIdx.x % PB) * KROW + 2 * HD;
+      *reinterpret_cast<u32x4v*>(pad) = u32x4v{0, 0, 0, 0};
+      *reinterpret_cast<u32x4v*>(pad + 16) = u32x4v{0, 0, 0, 0};
     }
-  }
-  for (int off = 8; off > 0; off >>= 1) {
-    wave_lo = min(wave_lo, __shfl_xor(wave_lo, off)); wave_hi = max(wave_hi, __shfl_xor(wave_hi, off));
-    all_lo = max(all_lo, __shfl_xor(all_lo, off)); all_hi = min(all_hi, __shfl_xor(all_hi, off));
-  }
-  const bool whole = __all(valid[0] && valid[CT - 1]);
-  int t0 = max(seg_lo, wave_lo & ~(BK - 1));
-  const int upto = min(seg_hi, wave_hi);
-  if (t0 < upto) {
-    Block blk;
-    for (; t0 < upto; t0 += BK) {
-      load_block(a, find_pages(a, table, t0, tile_lo, L, n, g), kvh, t0, tile_lo, L, n, g, blk);
-      const bool full = whole && t0 >= all_lo && t0 + BK - 1 <= all_hi && __all(blk.there);
-      if (full) attend<CT, true>(a, blk, t0, tile_lo, L, g, c);
-      else attend<CT, false>(a, blk, t0, tile_lo, L, g, c);
+    if (threadIdx.x < 4) flags[threadIdx.x] = 0;
+    // The pages of 32 blocks are held by the wave's lanes, one for every 16 keys, and a block's are read from there.
+    auto ask_pages = [&](int t0) { const int key = t0 + 16 * lane; return table[group_in(key, tile_lo, L) ? key >> a.page_shift : 0]; };
+    auto settle_pages = [&](int t0, int raw) { return group_in(t0 + 16 * lane, tile_lo, L) && (unsigned)raw < (unsigned)a.num_pages ? raw : -1; };
+    int pages = settle_pages(seg_lo, ask_pages(seg_lo)), more_pages = 0;
+    auto there_of = [&](int k) -> uint32_t {                  // bit i: the block's 16 keys i lie in a page
+      return (uint32_t)(__builtin_amdgcn_readlane(pages, (2 * k) & 63) >= 0) | (uint32_t)(__builtin_amdgcn_readlane(pages, (2 * k + 1) & 63) >= 0) << 1;
+    };
+    Staged s;
+    auto stage_load = [&](int k) {
+      const int off = (seg_lo + PB * k + 16 * group) & page_mask;
+      const int64_t at = (int64_t)max(__builtin_amdgcn_readlane(pages, (2 * k + group) & 63), 0) * a.Hkv + kvh;      // (page 0 is always there)
+      const uint8_t* kp = a.k + ((at << a.page_shift) + off + 8 * part) * HD;
+      const uint8_t* vp = a.v + ((at * HD + part * (HD / 2)) << a.page_shift) + off;
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        const uint32_t p = HD % 128 == 0 || lane + 64 * i < HD / 2 ? lane + 64 * i : 0;
+        s.k[i] = *reinterpret_cast<const u32x4v*>(kp + 16 * p);
+        s.v[i] = *reinterpret_cast<const u32x4v*>(vp + (p << a.page_shift));
+      }
+      const int64_t code = (at << (a.page_shift - 4)) + (off >> 4);
+      s.kcode = a.k_powers[code];
+      s.vcode = a.v_powers[code];
+    };
+    // A block's bytes into LDS, part j of 4 of them. Values of keys in front of tile_lo, or from L on, or in no page become zeros; a NaN among
+    // the others is reported.
+    uint32_t any_nan = 0;
+    // WHOLE: all of the block's groups lie in pages, between tile_lo and L.
+    auto stage_store = [&](auto whole_tag, int j, int t0, uint32_t there, char* buf) {
+      constexpr bool WHOLE = decltype(whole_tag)::value;
+      const int first = t0 + 16 * group;
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        const int p = lane + 64 * i;
+        if (j < 2) {
+          const float kp = power_of(s.kcode);
+          const int r = p / (HD / 16);       // of the wave's 8 keys: row 4 (2 group + part) + r % 4 of tile r / 4
+          char* kd = buf + (16 * (r >> 2) + 4 * wave + (r & 3)) * KROW + 32 * (p % (HD / 16));
+          if (HD % 128 == 0 || p < HD / 2) *reinterpret_cast<bf16x8*>(kd + 16 * j) = operand(s.k[i][2 * j], s.k[i][2 * j + 1], kp);
+        } else {
+          const int h = j - 2;
+          const float vp = power_of(s.vcode);
+          uint32_t w0 = s.v[i][2 * h], w1 = s.v[i][2 * h + 1];
+          if (!WHOLE && (!((there >> group) & 1) || first < tile_lo || first + 16 > L)) {
+            const int from = ((there >> group) & 1) ? tile_lo - first - 8 * h : 8, to = L - first - 8 * h;
+            const uint64_t upto = to >= 8 ? ~0ull : to <= 0 ? 0ull : (1ull << (8 * to)) - 1, below = from >= 8 ? ~0ull : from <= 0 ? 0ull : (1ull << (8 * from)) - 1;
+            const uint64_t keep = upto & ~below;
+            w0 &= (uint32_t)keep; w1 &= (uint32_t)(keep >> 32);
+          }
+          if (HD % 128 == 0 || p < HD / 2) {
+            any_nan |= ((w0 & 0x7f7f7f7fu) + 0x01010101u) | ((w1 & 0x7f7f7f7fu) + 0x01010101u);
+            *reinterpret_cast<bf16x8*>(buf + VBASE + (part * (HD / 2) + p) * VROW + 32 * group + 16 * h) = operand(w0, w1, vp);
+          }
+        }
+      }
+    };
+    auto report_nan = [&](int k) {
+      if (any_nan & 0x80808080u) flags[k & 3] = 1;
+      any_nan = 0;
+    };
+
+    // blocks 0 and 1 into LDS, block 2 on its way
+    uint32_t hist = 0;                        // two bits for every block from the current one on: its groups in pages
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (k < nblk) {
+        stage_load(k);
+        hist |= there_of(k) << (2 * k);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) stage_store(std::false_type{}, j, seg_lo + PB * k, there_of(k), lds_bytes + k * BUF);
+        report_nan(k);
+      }
+    if (2 < nblk) {
+      stage_load(2);
+      hist |= there_of(2) << 4;
+    }
+    __syncthreads();
+
+    const float sc = a.scale * LOG2E;
+    const uint32_t rd_k = n * KROW + 16 * g, rd_v = VBASE + n * VROW + 16 * g;
+    bf16x8 ka[2][KS];
+    auto read_keys = [&](uint32_t buf) {
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) ka[tt][ks] = *reinterpret_cast<const bf16x8*>(lds_bytes + buf + rd_k + 16 * tt * KROW + 64 * ks);
+    };
+    // product i of a block's scores: the chains of the key tiles and column tiles beside each other (one alone waits for itself)
+    auto score = [&](f32x4 (&st)[CT][2], int i) {
+      const int ct = i % CT, tt = i / CT % 2, ks = i / CT / 2;
+      st[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka[tt][ks], q[ct][ks], ks ? st[ct][tt] : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+    };
+    f32x4 st[CT][2];
+    read_keys(0);
+#pragma unroll
+    for (int i = 0; i < 2 * KS * CT; ++i) score(st, i);
+
+    uint32_t cur = 0, nxt = BUF, to = 2 * BUF;
+    // STEADY: every column of the wave sees every key of block k, all of them lie in pages, and so do block k + 2's, and there is a block
+    // k + 3; such a step has no branch but for a maximum that rises, a NaN and the next 32 pages.
+    auto step = [&](auto steady_tag, int k) {
+      constexpr bool STEADY = decltype(steady_tag)::value, FULL = STEADY;
+      const int t0 = seg_lo + PB * k;
+      const uint32_t there = hist & 3;
+      const bool nan = !FULL && flags[k & 3] != 0;
+      if (threadIdx.x == 0) flags[(k + 3) & 3] = 0;        // the block before this one's: nobody reads it any more, and the next to write it is a barrier away
+      read_keys(nxt);                         // (of the last block: what lies there is not used)
+      __builtin_amdgcn_sched_barrier(0);
+      bf16x8 va[DT];
+      // (half of the values' operands when half of the keys' have been used, the rest behind them: there are no registers for both)
+      auto read_values = [&](int from, int upto) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+          if (dt >= from && dt < upto) va[dt] = *reinterpret_cast<const bf16x8*>(lds_bytes + cur + rd_v + 16 * dt * VROW);
+      };
+      uint32_t seen[CT];
+      float sv[CT][8];
+      float top[CT];
+      bool rises = false;
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        if constexpr (!FULL) {
+          const int first = t0 + 8 * g;
+          const int from = max(c.lo[ct] - first, 0), upto = min(c.hi[ct] - first, 7);
+          seen[ct] = ((there >> (g >> 1)) & 1) && upto >= from && from < 8 ? (2u << upto) - (1u << from) : 0u;
+        }
+        top[ct] = NONE;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          sv[ct][i] = st[ct][i >> 2][i & 3];
+          if constexpr (!FULL) sv[ct][i] = (seen[ct] >> i) & 1 ? sv[ct][i] : NONE;
+          top[ct] = fmaxf(top[ct], sv[ct][i]);
+        }
+        rises = rises || (top[ct] > 0.5f * NONE && top[ct] * sc > c.m[ct] + RESCALE_STEP);
+      }
+      if (__any(rises)) {
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          const float t = max_of_column(top[ct]);
+          const float next = t > 0.5f * NONE ? t * sc : NONE;
+          if (next > c.m[ct] + RESCALE_STEP) {
+            const float f = __builtin_amdgcn_exp2f(c.m[ct] - next);
+            c.l[ct] *= f;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) c.acc[ct][dt][i] *= f;
+            c.m[ct] = next;
+          }
+        }
+      }
+      f32x4 sn[CT][2];
+      bf16x8 pb[CT];
+      float sum[CT], even[CT];
+      constexpr int NUMBERS = 8 * CT, SCORES = 2 * KS * CT;
+#pragma unroll
+      for (int i = 0; i < (NUMBERS > SCORES ? NUMBERS : SCORES); ++i) {
+        if (i == SCORES / 2) read_values(0, DT / 2);
+        if (i < SCORES) score(sn, i);
+        if (i < NUMBERS) {
+          const int ct = i % CT, e = i / CT;
+          float p = __builtin_amdgcn_exp2f(fmaf(sv[ct][e], sc, -c.m[ct]));
+          if constexpr (!FULL) p = (seen[ct] >> e) & 1 ? p : 0.f;      // while a column has seen no key, its reference point is NONE too
+          sum[ct] = e ? sum[ct] + p : p;
+          if (e & 1) { pb[ct][e - 1] = static_cast<bf16_t>(even[ct]); pb[ct][e] = static_cast<bf16_t>(p); }
+          else even[ct] = p;
+        }
+      }
+      read_values(DT / 2, DT);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) c.l[ct] += sum[ct];
+      if (!FULL && nan) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) values_with_nan<CT>(va[dt], seen, pb, dt, c);
+      } else {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) c.acc[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va[dt], pb[ct], c.acc[ct][dt], 0, 0, 0);
+          if constexpr (STEADY) {
+#pragma unroll
+            for (int j = dt * 4 / DT; j < (dt + 1) * 4 / DT; ++j) stage_store(std::true_type{}, j, 0, 3, lds_bytes + to);
+          }
+        }
+      }
+      if (!STEADY && k + 2 < nblk) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) stage_store(std::false_type{}, j, t0 + 2 * PB, (hist >> 4) & 3, lds_bytes + to);
+      }
+      if (STEADY || k + 2 < nblk) report_nan(k + 2);
+      hist >>= 2;
+      const int next = k + 3;
+      if (STEADY || next < nblk) {
+        // (stored whether they have changed or not: a store in each branch would put them into scratch memory)
+        int now = pages, later = more_pages;
+        if (__builtin_expect((next & 31) == 31, 0)) { asm volatile("" ::: "memory"); later = ask_pages(t0 + 4 * PB); }
+        if (__builtin_expect((next & 31) == 0, 0)) { asm volatile("" ::: "memory"); now = settle_pages(t0 + 3 * PB, later); }
+        pages = now; more_pages = later;
+        hist |= there_of(next) << 4;
+        stage_load(next);
+      }
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) { st[ct][0] = sn[ct][0]; st[ct][1] = sn[ct][1]; }
+      const uint32_t free = cur;
+      cur = nxt; nxt = to; to = free;
+      __syncthreads();
+    };
+    // (steady steps are a loop of their own: where the ways through a step meet, the sums would change their registers in every one)
+    auto steady = [&](int k) {
+      const int t0 = seg_lo + PB * k;
+      return k + 3 < nblk && t0 >= all_lo && t0 + PB - 1 <= all_hi && (hist & 0x33) == 0x33;
+    };
+    for (int k = 0; k < nblk; ++k) {
+      for (; steady(k); ++k) step(std::true_type{}, k);
+      step(std::false_type{}, k);
     }
   }
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     const float l = sum_of_column(c.l[ct]);
-    if (!valid[ct]) continue;
+    const int col = col0 + (wave * CT + ct) * 16 + n;
+    if (col >= q_len * a.G) continue;
+    const int tok = col / a.G, head = kvh * a.G + col - tok * a.G;
+    const int64_t row = q0 + tok;
     if (a.num_parts > 1) {
-      const int64_t at = (row[ct] * a.Hq + head[ct]) * a.num_parts + seg;
+      const int64_t at = (row * a.Hq + head) * a.num_parts + seg;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(a.part_o + at * HD + 16 * dt + 4 * g) = c.acc[ct][dt];
       if (g == 0) { a.part_ml[2 * at] = c.m[ct]; a.part_ml[2 * at + 1] = l; }
       continue;
     }
-    const float inv = inverse(with_sink(a, head[ct], c.m[ct], l));
-    bf16_t* o = a.out + row[ct] * a.out_stride + (int64_t)head[ct] * HD + 4 * g;
+    const float inv = inverse(with_sink(a, head, c.m[ct], l));
+    bf16_t* o = a.out + row * a.out_stride + (int64_t)head * HD + 4 * g;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       bf16x4 r;
@@ -541,16 +767,32 @@ extern "C" int me_attn8_decode(const void* q, int64_t q_stride, void* out, int64
 extern "C" int me_attn8_prompt(const void* q, int64_t q_stride, void* out, int64_t out_stride, const void* k, const void* v,
                                const void* k_powers, const void* v_powers, int64_t num_pages, const int32_t* tables, int table_stride,
                                int table_cols, const int32_t* contexts, const int32_t* cu, int64_t rows, int num_seqs, int Hq, int Hkv,
-                               int page, float scale, int window, int chunk, int part_keys, int num_parts, float* scratch,
+                               int page, float scale, int window, int chunk, int col_tiles, int part_keys, int num_parts, float* scratch,
                                const float* sinks, hipStream_t stream) {
   Attn8Args a;
   if (int rc = fill(a, q, q_stride, out, out_stride, k, v, k_powers, v_powers, num_pages, tables, table_stride, table_cols, contexts,
                     num_seqs, Hq, Hkv, page, scale, window, chunk, part_keys, num_parts, scratch, rows, sinks)) return rc;
   a.cu = cu;
-  constexpr int CT = 1;
-  const int64_t tiles = rows * a.G / (64 * CT) + num_seqs;
+  ME_CHECK(col_tiles == 1 || (col_tiles == 2 && HD <= 128), "attention_e4m3: %d column tiles per wave", col_tiles);
+  const int64_t tiles = rows * a.G / (64 * col_tiles) + num_seqs;
   ME_CHECK(rows >= 1 && rows * a.G < (1ll << 30) && tiles * Hkv < (1ll << 31), "attention_e4m3: too many tokens for one launch");
-  attn8_prompt_kernel<CT><<<dim3((unsigned)(tiles * Hkv), num_parts), 256, 0, stream>>>(a, (int)tiles);
+  const dim3 grid((unsigned)(tiles * Hkv), num_parts);
+  constexpr int lds = 3 * BUF + 16;
+#define PROMPT(CT)                                                                                                                   \
+  do {                                                                                                                               \
+    if (lds > 64 * 1024) {                                                                                                           \
+      hipError_t e = hipFuncSetAttribute((const void*)attn8_prompt_kernel<CT>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);     \
+      ME_CHECK(e == hipSuccess, "attention_e4m3: %d bytes of shared memory: %s", lds, hipGetErrorString(e));                         \
+    }                                                                                                                                \
+    attn8_prompt_kernel<CT><<<grid, 256, lds, stream>>>(a, (int)tiles);                                                              \
+  } while (0)
+  if constexpr (HD <= 128) {
+    if (col_tiles == 2) PROMPT(2);
+    else PROMPT(1);
+  } else {
+    PROMPT(1);
+  }
+#undef PROMPT
   ME_LAUNCH_CHECK();
   return join(a, rows, stream);
 }

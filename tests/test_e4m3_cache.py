@@ -141,13 +141,11 @@ def test_partitions_cover_the_keys(B, Hq, Hkv, ctx, span):
     worst = min(ctx, span + 63) if span else ctx
     assert part * parts >= worst
     for tokens in (2, 63, 489, 8192):
-        part, parts = ops.prompt_partitions_e4m3(tokens, 3, Hq, Hkv, 128, ctx, span)
-        assert parts >= 1
+        tiles, part, parts = ops.prompt_partitions_e4m3(tokens, 3, Hq, Hkv, 128, ctx, span)
+        assert parts >= 1 and tiles in (1, 2)
         if parts > 1:
-            assert part % 64 == 0 and part > 0 and part * parts >= ctx - 0 or span
-            rows = 256 // max(1, Hq // Hkv) + 1         # tokens of a tile: its keys begin with its first token's window
-            if span:
-                assert part * parts >= min(ctx, span + rows + 63)
+            rows = 64 * tiles // (Hq // Hkv) + 1         # tokens of a tile at most: its keys begin with its first token's window
+            assert part % 64 == 0 and part > 0 and part * parts >= (min(ctx, span + rows + 62) if span else ctx)
 
 
 def test_nan_is_the_only_number_that_is_not_finite():
