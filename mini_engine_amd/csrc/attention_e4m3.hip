@@ -16,7 +16,8 @@
 // Maxima, sums and accumulators are float32 and per column.
 //
 // Keys that a column does not see are replaced, never multiplied by zero: scores by "none", stored values by zero bytes where no
-// column sees them, and where some columns of a tile see a key whose value is NaN and others do not, only those that see it become NaN.
+// column sees them; and where some columns of a prompt's tile see a key whose value is NaN and others do not, the tile's columns are done
+// once more one by one.
 #include "e4m3.h"
 #include <type_traits>
 
@@ -207,29 +208,6 @@ __device__ __forceinline__ void softmax_tiles(const f32x4* st, float sc, int fir
   c.l[ct] += sum;
 }
 
-// The second product of one channel tile where a value may be NaN that some columns see and others do not: NaN counts as zero, and
-// whoever sees one becomes NaN (a product of what is NaN and what is seen counts them).
-template <int CT>
-__device__ __forceinline__ void values_with_nan(bf16x8 va, const uint32_t (&seen)[CT], const bf16x8 (&pb)[CT], int dt, Columns<CT>& c) {
-  bf16x8 bad;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const bool is = static_cast<float>(va[e]) != static_cast<float>(va[e]);
-    bad[e] = static_cast<bf16_t>(is ? 1.f : 0.f);
-    va[e] = is ? static_cast<bf16_t>(0.f) : va[e];
-  }
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    bf16x8 sees;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sees[e] = static_cast<bf16_t>((seen[ct] >> e) & 1 ? 1.f : 0.f);
-    const f32x4 count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bad, sees, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-    c.acc[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pb[ct], c.acc[ct][dt], 0, 0, 0);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c.acc[ct][dt][i] = count[i] > 0.f ? __uint_as_float(0x7fc00000u) : c.acc[ct][dt][i];
-  }
-}
-
 // One block out of registers, for a wave's single column tile. FULL: every column sees every key of it, and all of them lie in pages.
 // (Otherwise all columns see the same keys: what none of them sees is zeroed, and a NaN among the others is everybody's.)
 template <bool FULL>
@@ -344,31 +322,92 @@ __global__ void __launch_bounds__(256) attn8_decode_kernel(Attn8Args a) {
 // =====================================================================================
 // Portions of prompts. A tile is 64 CT columns of one request and key head; each of the 4 waves of its workgroup has 16 CT of them.
 // The workgroup walks the keys that its columns see in blocks of 32 (key 8 (m / 4) + 4 tt + m % 4 in row m of tile tt: lane (n, g) ends
-// with the 8 keys from 8 g on). A block's bytes are read once, three blocks ahead, and turned into bfloat16 once, two blocks ahead, in LDS,
-// from which every wave reads its operands (each wave all conversions for itself would be a third of its vector instructions). What a wave
-// reads of a block lies in one page under one power, so pages and addresses are scalars.
+// with the 8 keys from 8 g on). A block's bytes go to LDS by themselves (global_load_lds_dwordx4), five blocks ahead, and are turned into
+// bfloat16 once, two blocks ahead, from which every wave reads its operands (each wave all conversions for itself would be a third of its
+// vector instructions; bytes held in registers could be asked for one step ahead only, less than a trip to memory). What a wave brings of a
+// block lies in one page under one power, so pages, powers and addresses are scalars, and a lane turns into bfloat16 what it has brought itself.
 //   keys    [32][KROW]: row 16 tt + m, channels in order, and 16 bytes of padding, so that the 16 rows of a read lie in 16 different
 //           groups of banks. Channels from HD to the next 32 are zero.
 //   values  [HD][VROW]: 32 keys and the same padding.
 // Step k of the walk is a pipeline: beside the numbers of block k's softmax the products of block k + 1's scores, beside the products of
-// its values block k + 2's conversion. Three LDS buffers, one barrier a step.
+// its values block k + 2's conversion. One barrier a step. LDS: bytes of four blocks, keys of two, values of three.
 // Grid (tiles x key heads, segments): surplus tiles (the grid is made for the most there can be) exit.
 // =====================================================================================
 constexpr int PB = 32;                       // keys of a block
 constexpr int KS = (HD + 31) / 32;           // products of a tile of scores
 constexpr int KROW = 64 * KS + 16, VROW = 2 * PB + 16;                     // bytes
-constexpr int VBASE = PB * KROW, BUF = VBASE + HD * VROW;
+constexpr int KBUF = PB * KROW, VBUF = HD * VROW;
 constexpr int PIECES = (HD + 127) / 128;     // 16-byte pieces of keys (and of values) of a block that a lane brings
+constexpr int RAW = 4 * 1024 * PIECES;       // bytes of a block's keys (and of its values) as they come
+constexpr int AT_RAW = 0, AT_K = 8 * RAW, AT_V = AT_K + 2 * KBUF, AT_FLAGS = AT_V + 3 * VBUF, LDS_BYTES = AT_FLAGS + 16;
+static_assert(LDS_BYTES <= 160 * 1024 && (HD > 128 || 2 * LDS_BYTES <= 160 * 1024), "one workgroup to a compute unit, two up to head size 128");
 
-struct Staged {
-  u32x4v k[PIECES], v[PIECES];
-  uint32_t kcode, vcode;
-};
+// 64 x 16 bytes from base + voff (bytes, per lane) to LDS at lds_addr + 16 * lane. The write to m0 needs one wait state before an
+// instruction that reads it for an LDS address. base and lds_addr are the same in every lane.
+__device__ __forceinline__ void bring16(const uint8_t* base, uint32_t voff, uint32_t lds_addr) {
+  const uint64_t g = reinterpret_cast<uint64_t>(base);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(g >> 32)), lo = __builtin_amdgcn_readfirstlane((uint32_t)g);
+  const uint64_t from = (uint64_t)hi << 32 | lo;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds_addr)), "v"(voff), "s"(from) : "memory");
+}
+// All but the last N requests of this wave have landed.
+template <int N>
+__device__ __forceinline__ void brought() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+// The LDS writes of this wave done, every wave at the same point; requests to memory stay on their way.
+__device__ __forceinline__ void step_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// One column over the keys [lo, hi) that it sees, without a product of zero anywhere, key by key in plain float32: what a wave does with
+// its columns where a block that some of them see and others do not holds a value that is NaN. A lane scores every 64th key and has every
+// 64th channel.
+__device__ void one_column(const Attn8Args& a, const int32_t* table, int64_t row, int kvh, int head, int lo, int hi, int seg, int lane) {
+  const int mask = (1 << a.page_shift) - 1;
+  const bf16_t* q = a.q + row * a.q_stride + (int64_t)head * HD;
+  float m = NONE, l = 0.f, o[(HD + 63) / 64];
+#pragma unroll
+  for (int j = 0; j < (HD + 63) / 64; ++j) o[j] = 0.f;
+  for (int t0 = lo; t0 < hi; t0 += 64) {
+    const int key = t0 + lane;
+    const int page = key < hi ? table[key >> a.page_shift] : -1;
+    const bool sees = (unsigned)page < (unsigned)a.num_pages;
+    const int64_t at = (int64_t)(sees ? page : 0) * a.Hkv + kvh;
+    const int off = sees ? key & mask : 0;
+    const int64_t code = (at << (a.page_shift - 4)) + (off >> 4);
+    const float kp = power_of(a.k_powers[code]), vp = power_of(a.v_powers[code]);
+    float s = 0.f;
+    for (int d = 0; d < HD; ++d) s = fmaf(static_cast<float>(q[d]), __builtin_amdgcn_cvt_f32_fp8((int)a.k[((at << a.page_shift) + off) * HD + d], 0) * kp, s);
+    s = sees ? s * (a.scale * LOG2E) : NONE;
+    const float next = fmaxf(m, wave_max(s)), f = exp2f(m - next);
+    const float p = sees ? exp2f(s - next) : 0.f;
+    m = next;
+    l = l * f + wave_sum(p);
+#pragma unroll
+    for (int j = 0; j < (HD + 63) / 64; ++j) o[j] *= f;
+    for (int i = 0; i < 64; ++i) {
+      if (!__shfl((int)sees, i)) continue;
+      const float pi = __shfl(p, i), vpi = __shfl(vp, i);
+      const int64_t head_of = (int64_t)__shfl(page, i) * a.Hkv + kvh;
+      const int place = (t0 + i) & mask;
+#pragma unroll
+      for (int j = 0; j < (HD + 63) / 64; ++j)
+        if (lane + 64 * j < HD)
+          o[j] = fmaf(pi, __builtin_amdgcn_cvt_f32_fp8((int)a.v[((head_of * HD + lane + 64 * j) << a.page_shift) + place], 0) * vpi, o[j]);
+    }
+  }
+  const int64_t to = (row * a.Hq + head) * a.num_parts + seg;
+  const float inv = inverse(with_sink(a, head, m, l));
+#pragma unroll
+  for (int j = 0; j < (HD + 63) / 64; ++j)
+    if (lane + 64 * j < HD) {
+      if (a.num_parts > 1) a.part_o[to * HD + lane + 64 * j] = o[j];
+      else a.out[row * a.out_stride + (int64_t)head * HD + lane + 64 * j] = static_cast<bf16_t>(o[j] * inv);
+    }
+  if (a.num_parts > 1 && lane == 0) { a.part_ml[2 * to] = m; a.part_ml[2 * to + 1] = l; }
+}
 
 template <int CT>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 128 ? 2 : 1, HD <= 128 ? 2 : 1))) attn8_prompt_kernel(Attn8Args a, int tiles) {
-  extern __shared__ __align__(16) char lds_bytes[];        // three buffers, then a flag for each of four blocks in a row
-  int* flags = reinterpret_cast<int*>(lds_bytes + 3 * BUF);
+  extern __shared__ __align__(16) char lds_bytes[];        // (the flags: one for each of four blocks in a row)
+  int* flags = reinterpret_cast<int*>(lds_bytes + AT_FLAGS);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
   const int kvh = blockIdx.x % a.Hkv, tile = tiles - 1 - (int)(blockIdx.x / a.Hkv), seg = blockIdx.y;
@@ -394,6 +433,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
   Columns<CT> c;
   int all_lo = 0, all_hi = 0x7fffffff;
   bool whole = true;
+  int again = 0;                 // a block that some column may not see whole holds a value that is NaN
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     const int col = col0 + (wave * CT + ct) * 16 + n;
@@ -424,8 +464,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
   if (nblk > 0) {
     const int group = wave >> 1, part = wave & 1;             // this wave brings half of a block's 16 keys `group`: 8 keys, HD / 2 channels of values
     const int page_mask = (1 << a.page_shift) - 1;
-    if (HD % 32 != 0 && threadIdx.x < 3 * PB) {               // the channels that no head has: zeros, once
-      char* pad = lds_bytes + (threadIdx.x / PB) * BUF + (threadIdx.x % PB) * KROW + 2 * HD;
+    if (HD % 32 != 0 && threadIdx.x < 2 * PB) {               // the channels that no head has: zeros, once
+      char* pad = lds_bytes + AT_K + threadIdx.x * KROW + 2 * HD;
       *reinterpret_cast<u32x4v*>(pad) = u32x4v{0, 0, 0, 0};
       *reinterpret_cast<u32x4v*>(pad + 16) = u32x4v{0, 0, 0, 0};
     }
@@ -437,41 +477,57 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
     auto there_of = [&](int k) -> uint32_t {                  // bit i: the block's 16 keys i lie in a page
       return (uint32_t)(__builtin_amdgcn_readlane(pages, (2 * k) & 63) >= 0) | (uint32_t)(__builtin_amdgcn_readlane(pages, (2 * k + 1) & 63) >= 0) << 1;
     };
-    Staged s;
-    auto stage_load = [&](int k) {
+    // The powers of the same blocks, keys' and values' in one number, a lane for every 16 keys (asked for when the pages are known).
+    auto ask_codes = [&](int t0, int ids) -> int {
+      const int off = (t0 + 16 * lane) & page_mask;
+      const int64_t at = (((int64_t)max(ids, 0) * a.Hkv + kvh) << (a.page_shift - 4)) + (off >> 4);
+      return (int)a.k_powers[at] | (int)a.v_powers[at] << 8;
+    };
+    int codes = ask_codes(seg_lo, pages), more_codes = 0;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)lds_bytes;
+    const uint32_t mine = 16 * lane + 1024 * PIECES * wave;     // where this lane's pieces lie in a block's bytes
+    // block k's bytes to slot k % 4 (beyond the last block: page 0's, which is always there)
+    auto bring = [&](int k) {
       const int off = (seg_lo + PB * k + 16 * group) & page_mask;
-      const int64_t at = (int64_t)max(__builtin_amdgcn_readlane(pages, (2 * k + group) & 63), 0) * a.Hkv + kvh;      // (page 0 is always there)
+      const int64_t at = (int64_t)max(__builtin_amdgcn_readlane(pages, (2 * k + group) & 63), 0) * a.Hkv + kvh;
       const uint8_t* kp = a.k + ((at << a.page_shift) + off + 8 * part) * HD;
       const uint8_t* vp = a.v + ((at * HD + part * (HD / 2)) << a.page_shift) + off;
+      const uint32_t slot = lds0 + AT_RAW + (k & 3) * (2 * RAW) + 1024 * PIECES * wave;
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i)
+        if (HD % 128 == 0 || lane + 64 * i < HD / 2) {
+          bring16(kp + 1024 * i, 16 * lane, slot + 1024 * i);
+          bring16(vp + ((int64_t)(64 * i) << a.page_shift), (uint32_t)lane << a.page_shift, slot + RAW + 1024 * i);
+        }
+    };
+    u32x4v raw_k[PIECES], raw_v[PIECES];
+    auto read_raw = [&](int k) {
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
-        const uint32_t p = HD % 128 == 0 || lane + 64 * i < HD / 2 ? lane + 64 * i : 0;
-        s.k[i] = *reinterpret_cast<const u32x4v*>(kp + 16 * p);
-        s.v[i] = *reinterpret_cast<const u32x4v*>(vp + (p << a.page_shift));
+        const char* slot = lds_bytes + AT_RAW + (k & 3) * (2 * RAW) + mine + 1024 * i;
+        raw_k[i] = *reinterpret_cast<const u32x4v*>(slot);
+        raw_v[i] = *reinterpret_cast<const u32x4v*>(slot + RAW);
       }
-      const int64_t code = (at << (a.page_shift - 4)) + (off >> 4);
-      s.kcode = a.k_powers[code];
-      s.vcode = a.v_powers[code];
     };
-    // A block's bytes into LDS, part j of 4 of them. Values of keys in front of tile_lo, or from L on, or in no page become zeros; a NaN among
-    // the others is reported.
+    // Part j of 4 of a block as bfloat16. Values of keys in front of tile_lo, or from L on, or in no page become zeros; a NaN among the
+    // others is reported. WHOLE: all of the block's groups lie in pages, between tile_lo and L.
     uint32_t any_nan = 0;
-    // WHOLE: all of the block's groups lie in pages, between tile_lo and L.
-    auto stage_store = [&](auto whole_tag, int j, int t0, uint32_t there, char* buf) {
+    auto stage_store = [&](auto whole_tag, int j, int k, uint32_t there, char* kbuf, char* vbuf) {
       constexpr bool WHOLE = decltype(whole_tag)::value;
-      const int first = t0 + 16 * group;
+      const int first = seg_lo + PB * k + 16 * group;
+      const uint32_t code = __builtin_amdgcn_readlane(codes, (2 * k + group) & 63);
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
         const int p = lane + 64 * i;
         if (j < 2) {
-          const float kp = power_of(s.kcode);
+          const float kp = power_of(code & 0xff);
           const int r = p / (HD / 16);       // of the wave's 8 keys: row 4 (2 group + part) + r % 4 of tile r / 4
-          char* kd = buf + (16 * (r >> 2) + 4 * wave + (r & 3)) * KROW + 32 * (p % (HD / 16));
-          if (HD % 128 == 0 || p < HD / 2) *reinterpret_cast<bf16x8*>(kd + 16 * j) = operand(s.k[i][2 * j], s.k[i][2 * j + 1], kp);
+          char* kd = kbuf + (16 * (r >> 2) + 4 * wave + (r & 3)) * KROW + 32 * (p % (HD / 16));
+          if (HD % 128 == 0 || p < HD / 2) *reinterpret_cast<bf16x8*>(kd + 16 * j) = operand(raw_k[i][2 * j], raw_k[i][2 * j + 1], kp);
         } else {
           const int h = j - 2;
-          const float vp = power_of(s.vcode);
-          uint32_t w0 = s.v[i][2 * h], w1 = s.v[i][2 * h + 1];
+          const float vp = power_of(code >> 8);
+          uint32_t w0 = raw_v[i][2 * h], w1 = raw_v[i][2 * h + 1];
           if (!WHOLE && (!((there >> group) & 1) || first < tile_lo || first + 16 > L)) {
             const int from = ((there >> group) & 1) ? tile_lo - first - 8 * h : 8, to = L - first - 8 * h;
             const uint64_t upto = to >= 8 ? ~0ull : to <= 0 ? 0ull : (1ull << (8 * to)) - 1, below = from >= 8 ? ~0ull : from <= 0 ? 0ull : (1ull << (8 * from)) - 1;
@@ -480,36 +536,36 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
           }
           if (HD % 128 == 0 || p < HD / 2) {
             any_nan |= ((w0 & 0x7f7f7f7fu) + 0x01010101u) | ((w1 & 0x7f7f7f7fu) + 0x01010101u);
-            *reinterpret_cast<bf16x8*>(buf + VBASE + (part * (HD / 2) + p) * VROW + 32 * group + 16 * h) = operand(w0, w1, vp);
+            *reinterpret_cast<bf16x8*>(vbuf + (part * (HD / 2) + p) * VROW + 32 * group + 16 * h) = operand(w0, w1, vp);
           }
         }
       }
     };
     auto report_nan = [&](int k) {
-      if (any_nan & 0x80808080u) flags[k & 3] = 1;
+      if (__builtin_expect(any_nan & 0x80808080u, 0)) flags[k & 3] = 1;
       any_nan = 0;
     };
 
-    // blocks 0 and 1 into LDS, block 2 on its way
+    // blocks 0 and 1 as bfloat16, 2 to 4 on their way
     uint32_t hist = 0;                        // two bits for every block from the current one on: its groups in pages
-    __syncthreads();
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-      if (k < nblk) {
-        stage_load(k);
-        hist |= there_of(k) << (2 * k);
+    for (int k = 0; k < 4; ++k) bring(k);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) stage_store(std::false_type{}, j, seg_lo + PB * k, there_of(k), lds_bytes + k * BUF);
-        report_nan(k);
-      }
-    if (2 < nblk) {
-      stage_load(2);
-      hist |= there_of(2) << 4;
+    for (int k = 0; k < 5; ++k) hist |= there_of(k) << (2 * k);
+    step_barrier();                           // (the flags and the zeros)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (k == 0) brought<6 * PIECES>(); else brought<4 * PIECES>();
+      read_raw(k);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) stage_store(std::false_type{}, j, k, there_of(k), lds_bytes + AT_K + k * KBUF, lds_bytes + AT_V + k * VBUF);
+      report_nan(k);
     }
-    __syncthreads();
+    step_barrier();                           // (the bytes of block 0 have been read)
+    bring(4);
 
     const float sc = a.scale * LOG2E;
-    const uint32_t rd_k = n * KROW + 16 * g, rd_v = VBASE + n * VROW + 16 * g;
+    const uint32_t rd_k = AT_K + n * KROW + 16 * g, rd_v = AT_V + n * VROW + 16 * g;
     bf16x8 ka[2][KS];
     auto read_keys = [&](uint32_t buf) {
 #pragma unroll
@@ -524,19 +580,20 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
     };
     f32x4 st[CT][2];
     read_keys(0);
+    step_barrier();                           // (the first step writes block 2 over block 0's keys)
 #pragma unroll
     for (int i = 0; i < 2 * KS * CT; ++i) score(st, i);
 
-    uint32_t cur = 0, nxt = BUF, to = 2 * BUF;
-    // STEADY: every column of the wave sees every key of block k, all of them lie in pages, and so do block k + 2's, and there is a block
-    // k + 3; such a step has no branch but for a maximum that rises, a NaN and the next 32 pages.
+    uint32_t cur = 0, nxt = VBUF, to = 2 * VBUF;        // the values of blocks k, k + 1, k + 2
+    // STEADY: every column of the wave sees every key of block k, all of them lie in pages, and so do block k + 2's, which is not the last;
+    // such a step has no branch but for a maximum that rises, a NaN and what is held for the next 32 blocks.
     auto step = [&](auto steady_tag, int k) {
       constexpr bool STEADY = decltype(steady_tag)::value, FULL = STEADY;
       const int t0 = seg_lo + PB * k;
       const uint32_t there = hist & 3;
-      const bool nan = !FULL && flags[k & 3] != 0;
+      if constexpr (!FULL) again |= flags[k & 3];
       if (threadIdx.x == 0) flags[(k + 3) & 3] = 0;        // the block before this one's: nobody reads it any more, and the next to write it is a barrier away
-      read_keys(nxt);                         // (of the last block: what lies there is not used)
+      read_keys(((k + 1) & 1) * KBUF);         // (behind the last block: what lies there is not used)
       __builtin_amdgcn_sched_barrier(0);
       bf16x8 va[DT];
       // (half of the values' operands when half of the keys' have been used, the rest behind them: there are no registers for both)
@@ -564,9 +621,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
           if constexpr (!FULL) sv[ct][i] = (seen[ct] >> i) & 1 ? sv[ct][i] : NONE;
           top[ct] = fmaxf(top[ct], sv[ct][i]);
         }
-        rises = rises || (top[ct] > 0.5f * NONE && top[ct] * sc > c.m[ct] + RESCALE_STEP);
+        rises |= (top[ct] > 0.5f * NONE) & (top[ct] * sc > c.m[ct] + RESCALE_STEP);
       }
-      if (__any(rises)) {
+      if (__builtin_expect(__any(rises), 0)) {
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
           const float t = max_of_column(top[ct]);
@@ -599,54 +656,60 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
           else even[ct] = p;
         }
       }
+      brought<4 * PIECES>();                  // block k + 2; k + 3 and k + 4 are still on their way
+      read_raw(k + 2);
       read_values(DT / 2, DT);
+      char *kbuf = lds_bytes + AT_K + (k & 1) * KBUF, *vbuf = lds_bytes + AT_V + to;
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) c.l[ct] += sum[ct];
-      if (!FULL && nan) {
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) values_with_nan<CT>(va[dt], seen, pb, dt, c);
-      } else {
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
 #pragma unroll
           for (int ct = 0; ct < CT; ++ct) c.acc[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va[dt], pb[ct], c.acc[ct][dt], 0, 0, 0);
           if constexpr (STEADY) {
 #pragma unroll
-            for (int j = dt * 4 / DT; j < (dt + 1) * 4 / DT; ++j) stage_store(std::true_type{}, j, 0, 3, lds_bytes + to);
+            for (int j = dt * 4 / DT; j < (dt + 1) * 4 / DT; ++j) stage_store(std::true_type{}, j, k + 2, 3, kbuf, vbuf);
           }
         }
-      }
-      if (!STEADY && k + 2 < nblk) {
+      if constexpr (!STEADY) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) stage_store(std::false_type{}, j, t0 + 2 * PB, (hist >> 4) & 3, lds_bytes + to);
+        for (int j = 0; j < 4; ++j) stage_store(std::false_type{}, j, k + 2, (hist >> 4) & 3, kbuf, vbuf);
       }
-      if (STEADY || k + 2 < nblk) report_nan(k + 2);
-      hist >>= 2;
-      const int next = k + 3;
-      if (STEADY || next < nblk) {
-        // (stored whether they have changed or not: a store in each branch would put them into scratch memory)
-        int now = pages, later = more_pages;
-        if (__builtin_expect((next & 31) == 31, 0)) { asm volatile("" ::: "memory"); later = ask_pages(t0 + 4 * PB); }
-        if (__builtin_expect((next & 31) == 0, 0)) { asm volatile("" ::: "memory"); now = settle_pages(t0 + 3 * PB, later); }
-        pages = now; more_pages = later;
-        hist |= there_of(next) << 4;
-        stage_load(next);
-      }
+      report_nan(k + 2);
+      // (what is held for 32 blocks is stored whether it has changed or not: a store in each branch would put it into scratch memory)
+      const int next = k + 5, t_next = seg_lo + PB * next;
+      int now = pages, later = more_pages, now_codes = codes, later_codes = more_codes;
+      if (__builtin_expect((next & 31) == 31, 0)) { asm volatile("" ::: "memory"); later = ask_pages(t_next + PB); }
+      if (__builtin_expect((next & 31) == 0, 0)) { asm volatile("" ::: "memory"); now = settle_pages(t_next, later); later_codes = ask_codes(t_next, now); }
+      if (__builtin_expect((next & 31) == 2, 0)) now_codes = later_codes;          // the next step turns block k + 3 into bfloat16, the first of its 32
+      pages = now; more_pages = later; codes = now_codes; more_codes = later_codes;
+      hist = hist >> 2 | there_of(next) << 8;
+      bring(next);
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) { st[ct][0] = sn[ct][0]; st[ct][1] = sn[ct][1]; }
       const uint32_t free = cur;
       cur = nxt; nxt = to; to = free;
-      __syncthreads();
+      step_barrier();
     };
-    // (steady steps are a loop of their own: where the ways through a step meet, the sums would change their registers in every one)
-    auto steady = [&](int k) {
-      const int t0 = seg_lo + PB * k;
-      return k + 3 < nblk && t0 >= all_lo && t0 + PB - 1 <= all_hi && (hist & 0x33) == 0x33;
-    };
-    for (int k = 0; k < nblk; ++k) {
-      for (; steady(k); ++k) step(std::true_type{}, k);
-      step(std::false_type{}, k);
+    // Blocks are walked in ascending order: in front of the window's first whole block, those that the wave sees whole (steady as long as every
+    // group has its page), the rest. Loops of their own: where the ways through a step meet, the sums would change their registers.
+    const int first_steady = all_lo > seg_lo ? (all_lo - seg_lo + PB - 1) / PB : 0;
+    const int end_steady = all_hi >= seg_lo ? min((all_hi + 1 - seg_lo) / PB, nblk - 3) : 0;
+    int k = 0;
+    for (; k < min(first_steady, nblk); ++k) step(std::false_type{}, k);
+    for (; k < end_steady && (hist & 0x33) == 0x33; ++k) step(std::true_type{}, k);
+    for (; k < nblk; ++k) step(std::false_type{}, k);
+    brought<0>();                             // (what was asked for beyond the last block lands before the LDS is another workgroup's)
+  }
+  if (__builtin_expect(__any(again), 0)) {
+    // (zero times NaN: what such a block has added is of no use to the columns that do not see it)
+    for (int i = 0; i < 16 * CT; ++i) {
+      const int col = col0 + wave * CT * 16 + i;
+      if (col >= q_len * a.G) break;
+      const int tok = col / a.G;
+      one_column(a, table, q0 + tok, kvh, kvh * a.G + col - tok * a.G, max(seg_lo, first_seen(a, max(start + tok, 0))), min(seg_hi, start + tok + 1), seg, lane);
     }
+    return;
   }
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
@@ -718,6 +781,7 @@ static int fill(Attn8Args& a, const void* q, int64_t q_stride, void* out, int64_
                 int num_parts, float* scratch, int64_t rows, const float* sinks) {
   ME_CHECK(Hq >= 1 && Hkv >= 1 && Hq % Hkv == 0, "attention_e4m3: %d query heads are not a multiple of %d key heads", Hq, Hkv);
   ME_CHECK(page >= E4_BLOCK && (page & (page - 1)) == 0, "attention_e4m3: page size %d must be a power of two, 16 or more", page);
+  ME_CHECK(page <= 1 << 20, "attention_e4m3: page size %d beyond 2^20", page);
   ME_CHECK(num_pages >= 1 && num_pages * page < (1ll << 31), "attention_e4m3: %lld pages of %d tokens are more places than a slot can name", (long long)num_pages, page);
   ME_CHECK(q_stride % 8 == 0 && out_stride % 4 == 0, "attention_e4m3: token strides must keep 16-byte alignment");
   ME_CHECK(reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0 && reinterpret_cast<uintptr_t>(k) % 16 == 0 &&
@@ -777,7 +841,7 @@ extern "C" int me_attn8_prompt(const void* q, int64_t q_stride, void* out, int64
   const int64_t tiles = rows * a.G / (64 * col_tiles) + num_seqs;
   ME_CHECK(rows >= 1 && rows * a.G < (1ll << 30) && tiles * Hkv < (1ll << 31), "attention_e4m3: too many tokens for one launch");
   const dim3 grid((unsigned)(tiles * Hkv), num_parts);
-  constexpr int lds = 3 * BUF + 16;
+  constexpr int lds = LDS_BYTES;
 #define PROMPT(CT)                                                                                                                   \
   do {                                                                                                                               \
     if (lds > 64 * 1024) {                                                                                                           \
