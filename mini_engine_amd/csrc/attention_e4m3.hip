@@ -91,7 +91,9 @@ __device__ __forceinline__ bf16x8 operand(uint32_t w0, uint32_t w1, float power)
   const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, power, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, power, true);
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
-__device__ __forceinline__ float power_of(uint32_t code) { return __uint_as_float(min(max(code, (uint32_t)(E4_LEAST + E4_BIAS)), (uint32_t)(E4_MOST + E4_BIAS)) << 23); }
+// (a byte that no append has written may be anything)
+__device__ __forceinline__ uint32_t code_of(uint32_t byte) { return min(max(byte, (uint32_t)(E4_LEAST + E4_BIAS)), (uint32_t)(E4_MOST + E4_BIAS)); }
+__device__ __forceinline__ float power_of(uint32_t byte) { return __uint_as_float(code_of(byte) << 23); }
 
 // A block's keys and values as they lie in memory. Loads are unconditional: a lane whose keys are not to be read (at or past the
 // context, in front of what anybody sees, in a table entry without a page) reads page 0, which is always there.
@@ -326,20 +328,21 @@ __global__ void __launch_bounds__(256) attn8_decode_kernel(Attn8Args a) {
 // bfloat16 once, two blocks ahead, from which every wave reads its operands (each wave all conversions for itself would be a third of its
 // vector instructions; bytes held in registers could be asked for one step ahead only, less than a trip to memory). What a wave brings of a
 // block lies in one page under one power, so pages, powers and addresses are scalars, and a lane turns into bfloat16 what it has brought itself.
-//   keys    [32][KROW]: row 16 tt + m, channels in order, and 16 bytes of padding, so that the 16 rows of a read lie in 16 different
-//           groups of banks. Channels from HD to the next 32 are zero.
-//   values  [HD][VROW]: 32 keys and the same padding.
+//   keys    [pieces of 8 channels][row 16 tt + m] of 16 bytes: a read of 16 bytes a lane is worked off for lanes 0-3, 12-15 and 20-27
+//           together, then for the others of 32, which so lie in 16 different groups of banks whatever their lane group's piece. A wave writes
+//           rows of 4 groups of banks only; every second piece's rows therefore change places in fours (row ^ 4 (piece / 2 % 4)), which
+//           spreads the writes and leaves the reads, whose pieces come in such pairs, as they are. Channels from HD to the next 32 are zero.
+//   values  [8 keys][channel] of 16 bytes.
 // Step k of the walk is a pipeline: beside the numbers of block k's softmax the products of block k + 1's scores, beside the products of
 // its values block k + 2's conversion. One barrier a step. LDS: bytes of four blocks, keys of two, values of three.
 // Grid (tiles x key heads, segments): surplus tiles (the grid is made for the most there can be) exit.
 // =====================================================================================
 constexpr int PB = 32;                       // keys of a block
 constexpr int KS = (HD + 31) / 32;           // products of a tile of scores
-constexpr int KROW = 64 * KS + 16, VROW = 2 * PB + 16;                     // bytes
-constexpr int KBUF = PB * KROW, VBUF = HD * VROW;
+constexpr int KBUF = 4 * KS * PB * 16, VBUF = 4 * HD * 16;
 constexpr int PIECES = (HD + 127) / 128;     // 16-byte pieces of keys (and of values) of a block that a lane brings
 constexpr int RAW = 4 * 1024 * PIECES;       // bytes of a block's keys (and of its values) as they come
-constexpr int AT_RAW = 0, AT_K = 8 * RAW, AT_V = AT_K + 2 * KBUF, AT_FLAGS = AT_V + 3 * VBUF, LDS_BYTES = AT_FLAGS + 16;
+constexpr int AT_RAW = 0, AT_K = 8 * RAW, AT_V = AT_K + 2 * KBUF, AT_FLAGS = AT_V + 3 * VBUF, LDS_BYTES = AT_FLAGS + 16;      // (keys begin at multiples of 256)
 static_assert(LDS_BYTES <= 160 * 1024 && (HD > 128 || 2 * LDS_BYTES <= 160 * 1024), "one workgroup to a compute unit, two up to head size 128");
 
 // 64 x 16 bytes from base + voff (bytes, per lane) to LDS at lds_addr + 16 * lane. The write to m0 needs one wait state before an
@@ -406,8 +409,8 @@ __device__ void one_column(const Attn8Args& a, const int32_t* table, int64_t row
 
 template <int CT>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 128 ? 2 : 1, HD <= 128 ? 2 : 1))) attn8_prompt_kernel(Attn8Args a, int tiles) {
-  extern __shared__ __align__(16) char lds_bytes[];        // (the flags: one for each of four blocks in a row)
-  int* flags = reinterpret_cast<int*>(lds_bytes + AT_FLAGS);
+  extern __shared__ __align__(16) char lds_bytes[];
+  int* nan_flag = reinterpret_cast<int*>(lds_bytes + AT_FLAGS);      // a block that not every column sees whole holds a value that is NaN
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
   const int kvh = blockIdx.x % a.Hkv, tile = tiles - 1 - (int)(blockIdx.x / a.Hkv), seg = blockIdx.y;
@@ -431,9 +434,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
 
   bf16x8 q[CT][KS];
   Columns<CT> c;
-  int all_lo = 0, all_hi = 0x7fffffff;
-  bool whole = true;
-  int again = 0;                 // a block that some column may not see whole holds a value that is NaN
+  // keys that every column of the tile sees, and those that every column of this wave sees
+  const int tile_from = first_seen(a, max(start + last_tok / a.G, 0)), tile_upto = start + col0 / a.G;
+  int all_lo = 0, all_hi = 1 << 30;
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     const int col = col0 + (wave * CT + ct) * 16 + n;
@@ -454,50 +457,50 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
     }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) c.acc[ct][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    whole = whole && valid;
-    all_lo = max(all_lo, c.lo[ct]); all_hi = min(all_hi, c.hi[ct]);
+    all_lo = max(all_lo, valid ? c.lo[ct] : tile_from); all_hi = min(all_hi, valid ? c.hi[ct] : 1 << 30);      // (who is not there sees what the others see)
   }
   // (a wave's columns are in order: the first one that does not see a key is the last or the first of them)
   all_lo = __builtin_amdgcn_readlane(all_lo, 15); all_hi = __builtin_amdgcn_readlane(all_hi, 0);
-  if (!__all(whole)) all_hi = -1;
+  bool again = false;
 
   if (nblk > 0) {
     const int group = wave >> 1, part = wave & 1;             // this wave brings half of a block's 16 keys `group`: 8 keys, HD / 2 channels of values
     const int page_mask = (1 << a.page_shift) - 1;
-    if (HD % 32 != 0 && threadIdx.x < 2 * PB) {               // the channels that no head has: zeros, once
-      char* pad = lds_bytes + AT_K + threadIdx.x * KROW + 2 * HD;
-      *reinterpret_cast<u32x4v*>(pad) = u32x4v{0, 0, 0, 0};
-      *reinterpret_cast<u32x4v*>(pad + 16) = u32x4v{0, 0, 0, 0};
+    if (HD % 32 != 0 && threadIdx.x < 4 * PB) {               // the channels that no head has: zeros, once (two pieces of either buffer)
+      const int piece = HD / 8 + threadIdx.x / PB % 2, row = threadIdx.x % PB;
+      *reinterpret_cast<u32x4v*>(lds_bytes + AT_K + threadIdx.x / (2 * PB) * KBUF + (piece * PB + row) * 16) = u32x4v{0, 0, 0, 0};
     }
-    if (threadIdx.x < 4) flags[threadIdx.x] = 0;
+    if (threadIdx.x == 0) *nan_flag = 0;
     // The pages of 32 blocks are held by the wave's lanes, one for every 16 keys, and a block's are read from there.
     auto ask_pages = [&](int t0) { const int key = t0 + 16 * lane; return table[group_in(key, tile_lo, L) ? key >> a.page_shift : 0]; };
     auto settle_pages = [&](int t0, int raw) { return group_in(t0 + 16 * lane, tile_lo, L) && (unsigned)raw < (unsigned)a.num_pages ? raw : -1; };
     int pages = settle_pages(seg_lo, ask_pages(seg_lo)), more_pages = 0;
-    auto there_of = [&](int k) -> uint32_t {                  // bit i: the block's 16 keys i lie in a page
-      return (uint32_t)(__builtin_amdgcn_readlane(pages, (2 * k) & 63) >= 0) | (uint32_t)(__builtin_amdgcn_readlane(pages, (2 * k + 1) & 63) >= 0) << 1;
-    };
+    uint64_t held = __ballot(pages >= 0);
+    auto there_of = [&](int k) { return (uint32_t)(held >> ((2 * k) & 63)) & 3u; };      // bit i: the block's 16 keys i lie in a page
     // The powers of the same blocks, keys' and values' in one number, a lane for every 16 keys (asked for when the pages are known).
-    auto ask_codes = [&](int t0, int ids) -> int {
+    auto ask_codes = [&](int t0, int ids) -> uint32_t {
       const int off = (t0 + 16 * lane) & page_mask;
       const int64_t at = (((int64_t)max(ids, 0) * a.Hkv + kvh) << (a.page_shift - 4)) + (off >> 4);
-      return (int)a.k_powers[at] | (int)a.v_powers[at] << 8;
+      return code_of(a.k_powers[at]) << 23 | code_of(a.v_powers[at]) << 15;      // the power itself, and another 8 bits further right
     };
-    int codes = ask_codes(seg_lo, pages), more_codes = 0;
+    uint32_t codes = ask_codes(seg_lo, pages), more_codes = 0;
     const uint32_t lds0 = (uint32_t)(uintptr_t)lds_bytes;
     const uint32_t mine = 16 * lane + 1024 * PIECES * wave;     // where this lane's pieces lie in a block's bytes
-    // block k's bytes to slot k % 4 (beyond the last block: page 0's, which is always there)
+    // Block k's bytes to slot k % 4 (beyond the last block: page 0's, which is always there). A lane's keys: row lane % 8 of the wave's
+    // 8, 16 channels; its values: a channel.
+    const uint32_t page_bytes = (uint32_t)(a.Hkv * HD) << a.page_shift;
+    const uint8_t* k_head = a.k + (((int64_t)kvh << a.page_shift) + 8 * part) * HD;
+    const uint8_t* v_head = a.v + (((int64_t)kvh * HD + part * (HD / 2)) << a.page_shift);
+    const uint32_t k_lane = (lane & 7) * HD + (lane >> 3) * 16, v_lane = (uint32_t)lane << a.page_shift;
     auto bring = [&](int k) {
       const int off = (seg_lo + PB * k + 16 * group) & page_mask;
-      const int64_t at = (int64_t)max(__builtin_amdgcn_readlane(pages, (2 * k + group) & 63), 0) * a.Hkv + kvh;
-      const uint8_t* kp = a.k + ((at << a.page_shift) + off + 8 * part) * HD;
-      const uint8_t* vp = a.v + ((at * HD + part * (HD / 2)) << a.page_shift) + off;
+      const uint64_t at = (uint64_t)(uint32_t)max(__builtin_amdgcn_readlane(pages, (2 * k + group) & 63), 0) * page_bytes;
       const uint32_t slot = lds0 + AT_RAW + (k & 3) * (2 * RAW) + 1024 * PIECES * wave;
 #pragma unroll
       for (int i = 0; i < PIECES; ++i)
         if (HD % 128 == 0 || lane + 64 * i < HD / 2) {
-          bring16(kp + 1024 * i, 16 * lane, slot + 1024 * i);
-          bring16(vp + ((int64_t)(64 * i) << a.page_shift), (uint32_t)lane << a.page_shift, slot + RAW + 1024 * i);
+          bring16(k_head + at + off * HD + 128 * i, k_lane, slot + 1024 * i);
+          bring16(v_head + at + off + ((int64_t)(64 * i) << a.page_shift), v_lane, slot + RAW + 1024 * i);
         }
     };
     u32x4v raw_k[PIECES], raw_v[PIECES];
@@ -510,40 +513,41 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
       }
     };
     // Part j of 4 of a block as bfloat16. Values of keys in front of tile_lo, or from L on, or in no page become zeros; a NaN among the
-    // others is reported. WHOLE: all of the block's groups lie in pages, between tile_lo and L.
-    uint32_t any_nan = 0;
+    // others is reported. WHOLE: every column of the tile sees all of the block, and it lies in pages.
     auto stage_store = [&](auto whole_tag, int j, int k, uint32_t there, char* kbuf, char* vbuf) {
       constexpr bool WHOLE = decltype(whole_tag)::value;
       const int first = seg_lo + PB * k + 16 * group;
       const uint32_t code = __builtin_amdgcn_readlane(codes, (2 * k + group) & 63);
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
-        const int p = lane + 64 * i;
         if (j < 2) {
-          const float kp = power_of(code & 0xff);
-          const int r = p / (HD / 16);       // of the wave's 8 keys: row 4 (2 group + part) + r % 4 of tile r / 4
-          char* kd = kbuf + (16 * (r >> 2) + 4 * wave + (r & 3)) * KROW + 32 * (p % (HD / 16));
-          if (HD % 128 == 0 || p < HD / 2) *reinterpret_cast<bf16x8*>(kd + 16 * j) = operand(raw_k[i][2 * j], raw_k[i][2 * j + 1], kp);
+          // of the wave's 8 keys r: row 4 (2 group + part) + r % 4 of tile r / 4; channels 16 c + 8 j ..: piece 2 c + j
+          const float kp = __uint_as_float(code & 0x7f800000u);
+          const int r = lane & 7, c = (lane >> 3) + 8 * i;
+          char* kd = kbuf + (2 * c * PB + 16 * (r >> 2) + ((4 * wave + (r & 3)) ^ (4 * (c & 3)))) * 16;
+          if (HD % 128 == 0 || 16 * c < HD) *reinterpret_cast<bf16x8*>(kd + 16 * PB * j) = operand(raw_k[i][2 * j], raw_k[i][2 * j + 1], kp);
         } else {
-          const int h = j - 2;
-          const float vp = power_of(code >> 8);
+          const int h = j - 2, p = lane + 64 * i;
+          const float vp = __uint_as_float((code << 8) & 0x7f800000u);
           uint32_t w0 = raw_v[i][2 * h], w1 = raw_v[i][2 * h + 1];
-          if (!WHOLE && (!((there >> group) & 1) || first < tile_lo || first + 16 > L)) {
-            const int from = ((there >> group) & 1) ? tile_lo - first - 8 * h : 8, to = L - first - 8 * h;
-            const uint64_t upto = to >= 8 ? ~0ull : to <= 0 ? 0ull : (1ull << (8 * to)) - 1, below = from >= 8 ? ~0ull : from <= 0 ? 0ull : (1ull << (8 * from)) - 1;
-            const uint64_t keep = upto & ~below;
-            w0 &= (uint32_t)keep; w1 &= (uint32_t)(keep >> 32);
+          if constexpr (!WHOLE) {
+            if (!((there >> group) & 1) || first < tile_lo || first + 16 > L) {
+              const int from = ((there >> group) & 1) ? tile_lo - first - 8 * h : 8, to = L - first - 8 * h;
+              const uint64_t upto = to >= 8 ? ~0ull : to <= 0 ? 0ull : (1ull << (8 * to)) - 1, below = from >= 8 ? ~0ull : from <= 0 ? 0ull : (1ull << (8 * from)) - 1;
+              const uint64_t keep = upto & ~below;
+              w0 &= (uint32_t)keep; w1 &= (uint32_t)(keep >> 32);
+            }
           }
           if (HD % 128 == 0 || p < HD / 2) {
-            any_nan |= ((w0 & 0x7f7f7f7fu) + 0x01010101u) | ((w1 & 0x7f7f7f7fu) + 0x01010101u);
-            *reinterpret_cast<bf16x8*>(vbuf + (part * (HD / 2) + p) * VROW + 32 * group + 16 * h) = operand(w0, w1, vp);
+            if constexpr (!WHOLE) {
+              // all seven lower bits of a byte
+              const uint32_t nan = (((w0 & 0x7f7f7f7fu) + 0x01010101u) | ((w1 & 0x7f7f7f7fu) + 0x01010101u)) & 0x80808080u;
+              if (__builtin_expect(nan != 0, 0)) *nan_flag = 1;
+            }
+            *reinterpret_cast<bf16x8*>(vbuf + ((2 * group + h) * HD + part * (HD / 2) + p) * 16) = operand(w0, w1, vp);
           }
         }
       }
-    };
-    auto report_nan = [&](int k) {
-      if (__builtin_expect(any_nan & 0x80808080u, 0)) flags[k & 3] = 1;
-      any_nan = 0;
     };
 
     // blocks 0 and 1 as bfloat16, 2 to 4 on their way
@@ -559,19 +563,20 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
       read_raw(k);
 #pragma unroll
       for (int j = 0; j < 4; ++j) stage_store(std::false_type{}, j, k, there_of(k), lds_bytes + AT_K + k * KBUF, lds_bytes + AT_V + k * VBUF);
-      report_nan(k);
     }
     step_barrier();                           // (the bytes of block 0 have been read)
     bring(4);
 
     const float sc = a.scale * LOG2E;
-    const uint32_t rd_k = AT_K + n * KROW + 16 * g, rd_v = AT_V + n * VROW + 16 * g;
+    const uint32_t rd_v = AT_V + (g * HD + n) * 16;
+    // pieces 4 ks + g: rows change places by 4 (2 (ks % 2) + g / 2)
+    const uint32_t rd_k[2] = {(uint32_t)(AT_K + (g * PB + (n ^ (4 * (g >> 1)))) * 16), (uint32_t)(AT_K + (g * PB + (n ^ (8 + 4 * (g >> 1)))) * 16)};
     bf16x8 ka[2][KS];
     auto read_keys = [&](uint32_t buf) {
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) ka[tt][ks] = *reinterpret_cast<const bf16x8*>(lds_bytes + buf + rd_k + 16 * tt * KROW + 64 * ks);
+        for (int ks = 0; ks < KS; ++ks) ka[tt][ks] = *reinterpret_cast<const bf16x8*>(lds_bytes + buf + rd_k[ks & 1] + (4 * ks * PB + 16 * tt) * 16);
     };
     // product i of a block's scores: the chains of the key tiles and column tiles beside each other (one alone waits for itself)
     auto score = [&](f32x4 (&st)[CT][2], int i) {
@@ -585,14 +590,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
     for (int i = 0; i < 2 * KS * CT; ++i) score(st, i);
 
     uint32_t cur = 0, nxt = VBUF, to = 2 * VBUF;        // the values of blocks k, k + 1, k + 2
-    // STEADY: every column of the wave sees every key of block k, all of them lie in pages, and so do block k + 2's, which is not the last;
-    // such a step has no branch but for a maximum that rises, a NaN and what is held for the next 32 blocks.
+    // STEADY: every column of the wave sees every key of block k, every one of the tile those of block k + 2, and both lie in pages; such a
+    // step has no branch but for a maximum that rises and for what is held for the next 32 blocks.
     auto step = [&](auto steady_tag, int k) {
       constexpr bool STEADY = decltype(steady_tag)::value, FULL = STEADY;
       const int t0 = seg_lo + PB * k;
       const uint32_t there = hist & 3;
-      if constexpr (!FULL) again |= flags[k & 3];
-      if (threadIdx.x == 0) flags[(k + 3) & 3] = 0;        // the block before this one's: nobody reads it any more, and the next to write it is a barrier away
       read_keys(((k + 1) & 1) * KBUF);         // (behind the last block: what lies there is not used)
       __builtin_amdgcn_sched_barrier(0);
       bf16x8 va[DT];
@@ -601,7 +604,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
-          if (dt >= from && dt < upto) va[dt] = *reinterpret_cast<const bf16x8*>(lds_bytes + cur + rd_v + 16 * dt * VROW);
+          if (dt >= from && dt < upto) va[dt] = *reinterpret_cast<const bf16x8*>(lds_bytes + cur + rd_v + 256 * dt);
       };
       uint32_t seen[CT];
       float sv[CT][8];
@@ -675,12 +678,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
 #pragma unroll
         for (int j = 0; j < 4; ++j) stage_store(std::false_type{}, j, k + 2, (hist >> 4) & 3, kbuf, vbuf);
       }
-      report_nan(k + 2);
       // (what is held for 32 blocks is stored whether it has changed or not: a store in each branch would put it into scratch memory)
       const int next = k + 5, t_next = seg_lo + PB * next;
-      int now = pages, later = more_pages, now_codes = codes, later_codes = more_codes;
+      int now = pages, later = more_pages;
+      uint32_t now_codes = codes, later_codes = more_codes;
       if (__builtin_expect((next & 31) == 31, 0)) { asm volatile("" ::: "memory"); later = ask_pages(t_next + PB); }
-      if (__builtin_expect((next & 31) == 0, 0)) { asm volatile("" ::: "memory"); now = settle_pages(t_next, later); later_codes = ask_codes(t_next, now); }
+      if (__builtin_expect((next & 31) == 0, 0)) { asm volatile("" ::: "memory"); now = settle_pages(t_next, later); later_codes = ask_codes(t_next, now); held = __ballot(now >= 0); }
       if (__builtin_expect((next & 31) == 2, 0)) now_codes = later_codes;          // the next step turns block k + 3 into bfloat16, the first of its 32
       pages = now; more_pages = later; codes = now_codes; more_codes = later_codes;
       hist = hist >> 2 | there_of(next) << 8;
@@ -693,15 +696,16 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
     };
     // Blocks are walked in ascending order: in front of the window's first whole block, those that the wave sees whole (steady as long as every
     // group has its page), the rest. Loops of their own: where the ways through a step meet, the sums would change their registers.
-    const int first_steady = all_lo > seg_lo ? (all_lo - seg_lo + PB - 1) / PB : 0;
-    const int end_steady = all_hi >= seg_lo ? min((all_hi + 1 - seg_lo) / PB, nblk - 3) : 0;
+    const int first_steady = max(all_lo - seg_lo + PB - 1, 0) / PB, first_whole = max(tile_from - seg_lo + PB - 1, 0) / PB;
+    const int end_steady = all_hi >= seg_lo && tile_upto >= seg_lo ? min(min((all_hi + 1 - seg_lo) / PB, (tile_upto + 1 - seg_lo) / PB - 2), nblk) : 0;
     int k = 0;
-    for (; k < min(first_steady, nblk); ++k) step(std::false_type{}, k);
+    for (; k < min(max(first_steady, first_whole - 2), nblk); ++k) step(std::false_type{}, k);
     for (; k < end_steady && (hist & 0x33) == 0x33; ++k) step(std::true_type{}, k);
     for (; k < nblk; ++k) step(std::false_type{}, k);
     brought<0>();                             // (what was asked for beyond the last block lands before the LDS is another workgroup's)
+    again = *nan_flag != 0;
   }
-  if (__builtin_expect(__any(again), 0)) {
+  if (__builtin_expect(again, 0)) {
     // (zero times NaN: what such a block has added is of no use to the columns that do not see it)
     for (int i = 0; i < 16 * CT; ++i) {
       const int col = col0 + wave * CT * 16 + i;
@@ -781,7 +785,7 @@ static int fill(Attn8Args& a, const void* q, int64_t q_stride, void* out, int64_
                 int num_parts, float* scratch, int64_t rows, const float* sinks) {
   ME_CHECK(Hq >= 1 && Hkv >= 1 && Hq % Hkv == 0, "attention_e4m3: %d query heads are not a multiple of %d key heads", Hq, Hkv);
   ME_CHECK(page >= E4_BLOCK && (page & (page - 1)) == 0, "attention_e4m3: page size %d must be a power of two, 16 or more", page);
-  ME_CHECK(page <= 1 << 20, "attention_e4m3: page size %d beyond 2^20", page);
+  ME_CHECK((int64_t)Hkv * page * HD < (1ll << 31), "attention_e4m3: a page of %d tokens and %d heads is beyond 2^31 bytes", page, Hkv);
   ME_CHECK(num_pages >= 1 && num_pages * page < (1ll << 31), "attention_e4m3: %lld pages of %d tokens are more places than a slot can name", (long long)num_pages, page);
   ME_CHECK(q_stride % 8 == 0 && out_stride % 4 == 0, "attention_e4m3: token strides must keep 16-byte alignment");
   ME_CHECK(reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0 && reinterpret_cast<uintptr_t>(k) % 16 == 0 &&
