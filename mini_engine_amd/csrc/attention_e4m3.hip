@@ -322,24 +322,28 @@ __global__ void __launch_bounds__(256) attn8_decode_kernel(Attn8Args a) {
 }
 
 // =====================================================================================
-// Portions of prompts. A tile is 64 CT columns of one request and key head; each of the 4 waves of its workgroup has 16 CT of them.
-// The workgroup walks the keys that its columns see in blocks of 32 (key 8 (m / 4) + 4 tt + m % 4 in row m of tile tt: lane (n, g) ends
-// with the 8 keys from 8 g on). A block's bytes go to LDS by themselves (global_load_lds_dwordx4), five blocks ahead, and are turned into
-// bfloat16 once, two blocks ahead, from which every wave reads its operands (each wave all conversions for itself would be a third of its
-// vector instructions; bytes held in registers could be asked for one step ahead only, less than a trip to memory). What a wave brings of a
-// block lies in one page under one power, so pages, powers and addresses are scalars, and a lane turns into bfloat16 what it has brought itself.
-//   keys    [pieces of 8 channels][row 16 tt + m] of 16 bytes: a read of 16 bytes a lane is worked off for lanes 0-3, 12-15 and 20-27
-//           together, then for the others of 32, which so lie in 16 different groups of banks whatever their lane group's piece. A wave writes
-//           rows of 4 groups of banks only; every second piece's rows therefore change places in fours (row ^ 4 (piece / 2 % 4)), which
-//           spreads the writes and leaves the reads, whose pieces come in such pairs, as they are. Channels from HD to the next 32 are zero.
+// Portions of prompts. A tile is 128 columns of one request and key head; each of the 4 waves of its workgroup has 32 of them, a column to
+// two lanes (l and l ^ 32). The workgroup walks the keys that its columns see in blocks of 32 with v_mfma_f32_32x32x16_bf16 (half as many
+// instructions as tiles of 16 x 16 take, and one column's state to a lane instead of two). Row r of a tile of scores stands for the key whose bits 2
+// and 3 are exchanged: lane l then holds keys 8 h .. 8 h + 7 and 16 + 8 h .. of its column (h = l / 32), the values' operand as it is.
+// A block's bytes go to LDS by themselves (global_load_lds_dwordx4), five blocks ahead, and are turned into bfloat16 once, two blocks
+// ahead, from which every wave reads its operands (each wave all conversions for itself would be a third of its vector instructions; bytes
+// held in registers could be asked for one step ahead only, less than a trip to memory). What a wave brings of a block lies in one page
+// under one power, so pages, powers and addresses are scalars, and a lane turns into bfloat16 what it has brought itself.
+//   keys    [pieces of 8 channels][32 rows] of 16 bytes: a read of 16 bytes a lane is worked off for lanes 0-3, 12-15 and 20-27 together,
+//           then for the others of 32, which so lie in 16 different groups of banks. A wave writes two fours of a piece's rows; their fours
+//           change places in every second pair of pieces (row ^ 4), which spreads the writes over all banks and leaves the reads as they are.
 //   values  [8 keys][channel] of 16 bytes.
 // Step k of the walk is a pipeline: beside the numbers of block k's softmax the products of block k + 1's scores, beside the products of
 // its values block k + 2's conversion. One barrier a step. LDS: bytes of four blocks, keys of two, values of three.
 // Grid (tiles x key heads, segments): surplus tiles (the grid is made for the most there can be) exit.
 // =====================================================================================
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+constexpr int COLS = 128;                    // columns of a tile
 constexpr int PB = 32;                       // keys of a block
-constexpr int KS = (HD + 31) / 32;           // products of a tile of scores
-constexpr int KBUF = 4 * KS * PB * 16, VBUF = 4 * HD * 16;
+constexpr int KS = HD / 16;                  // products of a tile of scores
+constexpr int DC = (HD + 31) / 32;           // channel tiles of the values
+constexpr int KBUF = 2 * KS * PB * 16, VBUF = 4 * DC * 32 * 16;
 constexpr int PIECES = (HD + 127) / 128;     // 16-byte pieces of keys (and of values) of a block that a lane brings
 constexpr int RAW = 4 * 1024 * PIECES;       // bytes of a block's keys (and of its values) as they come
 constexpr int AT_RAW = 0, AT_K = 8 * RAW, AT_V = AT_K + 2 * KBUF, AT_FLAGS = AT_V + 3 * VBUF, LDS_BYTES = AT_FLAGS + 16;      // (keys begin at multiples of 256)
@@ -407,14 +411,12 @@ __device__ void one_column(const Attn8Args& a, const int32_t* table, int64_t row
   if (a.num_parts > 1 && lane == 0) { a.part_ml[2 * to] = m; a.part_ml[2 * to + 1] = l; }
 }
 
-template <int CT>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 128 ? 2 : 1, HD <= 128 ? 2 : 1))) attn8_prompt_kernel(Attn8Args a, int tiles) {
   extern __shared__ __align__(16) char lds_bytes[];
   int* nan_flag = reinterpret_cast<int*>(lds_bytes + AT_FLAGS);      // a block that not every column sees whole holds a value that is NaN
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n = lane & 15, g = lane >> 4;
+  const int n = lane & 31, h = lane >> 5;
   const int kvh = blockIdx.x % a.Hkv, tile = tiles - 1 - (int)(blockIdx.x / a.Hkv), seg = blockIdx.y;
-  constexpr int COLS = 64 * CT;
   // request b has the tiles from cu[b] * G / COLS + b on
   int b = 0, end = a.num_seqs;
   while (end - b > 1) {
@@ -431,45 +433,38 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
   const int tile_lo = first_seen(a, max(start + col0 / a.G, 0)), tile_hi = start + last_tok / a.G + 1;
   const int seg_lo = (tile_lo & ~(BK - 1)) + seg * a.part_keys, seg_hi = seg + 1 < a.num_parts ? min(tile_hi, seg_lo + a.part_keys) : tile_hi;
   const int nblk = (seg_hi - seg_lo + PB - 1) / PB;           // (none: not above 0)
-
-  bf16x8 q[CT][KS];
-  Columns<CT> c;
-  // keys that every column of the tile sees, and those that every column of this wave sees
+  // keys that every column of the tile sees
   const int tile_from = first_seen(a, max(start + last_tok / a.G, 0)), tile_upto = start + col0 / a.G;
-  int all_lo = 0, all_hi = 1 << 30;
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    const int col = col0 + (wave * CT + ct) * 16 + n;
-    const bool valid = col < q_len * a.G;
-    const int tok = valid ? col / a.G : 0;
-    const int head = kvh * a.G + (valid ? col - tok * a.G : 0);
-    c.m[ct] = NONE; c.l[ct] = 0.f;
-    c.hi[ct] = valid ? start + tok : -1;
-    c.lo[ct] = valid ? first_seen(a, max(start + tok, 0)) : 0;
-    const bf16_t* row = a.q + (q0 + tok) * a.q_stride + (int64_t)head * HD;
+
+  const int col = col0 + 32 * wave + n;
+  const bool valid = col < q_len * a.G;
+  const int tok = valid ? col / a.G : 0, head = kvh * a.G + (valid ? col - tok * a.G : 0);
+  const int64_t row = q0 + tok;
+  float m = NONE, l = 0.f;
+  const int lo = valid ? first_seen(a, max(start + tok, 0)) : 0, hi = valid ? start + tok : -1;      // the keys that the column sees
+  bf16x8 q[KS];
+  {
+    const bf16_t* from = a.q + row * a.q_stride + (int64_t)head * HD + 8 * h;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      const bool in = HD % 32 == 0 || 32 * ks + 8 * g < HD;
-      bf16x8 x = *reinterpret_cast<const bf16x8*>(row + (in ? 32 * ks + 8 * g : 0));
+      bf16x8 x = *reinterpret_cast<const bf16x8*>(from + 16 * ks);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = valid && in ? x[e] : static_cast<bf16_t>(0.f);
-      q[ct][ks] = x;
+      for (int e = 0; e < 8; ++e) x[e] = valid ? x[e] : static_cast<bf16_t>(0.f);
+      q[ks] = x;
     }
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) c.acc[ct][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    all_lo = max(all_lo, valid ? c.lo[ct] : tile_from); all_hi = min(all_hi, valid ? c.hi[ct] : 1 << 30);      // (who is not there sees what the others see)
   }
-  // (a wave's columns are in order: the first one that does not see a key is the last or the first of them)
-  all_lo = __builtin_amdgcn_readlane(all_lo, 15); all_hi = __builtin_amdgcn_readlane(all_hi, 0);
+  f32x16 acc[DC];
+#pragma unroll
+  for (int dt = 0; dt < DC; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
+  // the keys that every column of the wave sees: columns are in order, and who is not there sees what the others see
+  const int all_lo = __builtin_amdgcn_readlane(valid ? lo : tile_from, 31), all_hi = __builtin_amdgcn_readlane(valid ? hi : 1 << 30, 0);
   bool again = false;
 
   if (nblk > 0) {
     const int group = wave >> 1, part = wave & 1;             // this wave brings half of a block's 16 keys `group`: 8 keys, HD / 2 channels of values
     const int page_mask = (1 << a.page_shift) - 1;
-    if (HD % 32 != 0 && threadIdx.x < 4 * PB) {               // the channels that no head has: zeros, once (two pieces of either buffer)
-      const int piece = HD / 8 + threadIdx.x / PB % 2, row = threadIdx.x % PB;
-      *reinterpret_cast<u32x4v*>(lds_bytes + AT_K + threadIdx.x / (2 * PB) * KBUF + (piece * PB + row) * 16) = u32x4v{0, 0, 0, 0};
-    }
     if (threadIdx.x == 0) *nan_flag = 0;
     // The pages of 32 blocks are held by the wave's lanes, one for every 16 keys, and a block's are read from there.
     auto ask_pages = [&](int t0) { const int key = t0 + 16 * lane; return table[group_in(key, tile_lo, L) ? key >> a.page_shift : 0]; };
@@ -521,18 +516,18 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
         if (j < 2) {
-          // of the wave's 8 keys r: row 4 (2 group + part) + r % 4 of tile r / 4; channels 16 c + 8 j ..: piece 2 c + j
+          // of the wave's 8 keys 16 group + 8 part + r: row 16 group + 8 (r / 4) + 4 part + r % 4; channels 16 c + 8 j ..: piece 2 c + j
           const float kp = __uint_as_float(code & 0x7f800000u);
           const int r = lane & 7, c = (lane >> 3) + 8 * i;
-          char* kd = kbuf + (2 * c * PB + 16 * (r >> 2) + ((4 * wave + (r & 3)) ^ (4 * (c & 3)))) * 16;
+          char* kd = kbuf + (2 * c * PB + ((16 * group + 8 * (r >> 2) + 4 * part + (r & 3)) ^ (4 * ((c >> 1) & 1)))) * 16;
           if (HD % 128 == 0 || 16 * c < HD) *reinterpret_cast<bf16x8*>(kd + 16 * PB * j) = operand(raw_k[i][2 * j], raw_k[i][2 * j + 1], kp);
         } else {
-          const int h = j - 2, p = lane + 64 * i;
+          const int half = j - 2, p = lane + 64 * i;
           const float vp = __uint_as_float((code << 8) & 0x7f800000u);
-          uint32_t w0 = raw_v[i][2 * h], w1 = raw_v[i][2 * h + 1];
+          uint32_t w0 = raw_v[i][2 * half], w1 = raw_v[i][2 * half + 1];
           if constexpr (!WHOLE) {
             if (!((there >> group) & 1) || first < tile_lo || first + 16 > L) {
-              const int from = ((there >> group) & 1) ? tile_lo - first - 8 * h : 8, to = L - first - 8 * h;
+              const int from = ((there >> group) & 1) ? tile_lo - first - 8 * half : 8, to = L - first - 8 * half;
               const uint64_t upto = to >= 8 ? ~0ull : to <= 0 ? 0ull : (1ull << (8 * to)) - 1, below = from >= 8 ? ~0ull : from <= 0 ? 0ull : (1ull << (8 * from)) - 1;
               const uint64_t keep = upto & ~below;
               w0 &= (uint32_t)keep; w1 &= (uint32_t)(keep >> 32);
@@ -544,7 +539,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
               const uint32_t nan = (((w0 & 0x7f7f7f7fu) + 0x01010101u) | ((w1 & 0x7f7f7f7fu) + 0x01010101u)) & 0x80808080u;
               if (__builtin_expect(nan != 0, 0)) *nan_flag = 1;
             }
-            *reinterpret_cast<bf16x8*>(vbuf + ((2 * group + h) * HD + part * (HD / 2) + p) * 16) = operand(w0, w1, vp);
+            *reinterpret_cast<bf16x8*>(vbuf + ((2 * group + half) * (32 * DC) + part * (HD / 2) + p) * 16) = operand(w0, w1, vp);
           }
         }
       }
@@ -568,26 +563,20 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
     bring(4);
 
     const float sc = a.scale * LOG2E;
-    const uint32_t rd_v = AT_V + (g * HD + n) * 16;
-    // pieces 4 ks + g: rows change places by 4 (2 (ks % 2) + g / 2)
-    const uint32_t rd_k[2] = {(uint32_t)(AT_K + (g * PB + (n ^ (4 * (g >> 1)))) * 16), (uint32_t)(AT_K + (g * PB + (n ^ (8 + 4 * (g >> 1)))) * 16)};
-    bf16x8 ka[2][KS];
+    const uint32_t rd_v = AT_V + (32 * DC * h + n) * 16;
+    // pieces 2 ks + h: the rows' fours change places where ks / 2 is odd
+    const uint32_t rd_k[2] = {(uint32_t)(AT_K + (h * PB + n) * 16), (uint32_t)(AT_K + (h * PB + (n ^ 4)) * 16)};
+    bf16x8 ka[KS];
     auto read_keys = [&](uint32_t buf) {
 #pragma unroll
-      for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) ka[tt][ks] = *reinterpret_cast<const bf16x8*>(lds_bytes + buf + rd_k[ks & 1] + (4 * ks * PB + 16 * tt) * 16);
+      for (int ks = 0; ks < KS; ++ks) ka[ks] = *reinterpret_cast<const bf16x8*>(lds_bytes + buf + rd_k[(ks >> 1) & 1] + 2 * ks * PB * 16);
     };
-    // product i of a block's scores: the chains of the key tiles and column tiles beside each other (one alone waits for itself)
-    auto score = [&](f32x4 (&st)[CT][2], int i) {
-      const int ct = i % CT, tt = i / CT % 2, ks = i / CT / 2;
-      st[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka[tt][ks], q[ct][ks], ks ? st[ct][tt] : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-    };
-    f32x4 st[CT][2];
+    const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    f32x16 st;                                // the scores of the block whose softmax comes next
     read_keys(0);
     step_barrier();                           // (the first step writes block 2 over block 0's keys)
 #pragma unroll
-    for (int i = 0; i < 2 * KS * CT; ++i) score(st, i);
+    for (int ks = 0; ks < KS; ++ks) st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[ks], q[ks], ks ? st : zero, 0, 0, 0);
 
     uint32_t cur = 0, nxt = VBUF, to = 2 * VBUF;        // the values of blocks k, k + 1, k + 2
     // STEADY: every column of the wave sees every key of block k, every one of the tile those of block k + 2, and both lie in pages; such a
@@ -598,82 +587,70 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
       const uint32_t there = hist & 3;
       read_keys(((k + 1) & 1) * KBUF);         // (behind the last block: what lies there is not used)
       __builtin_amdgcn_sched_barrier(0);
-      bf16x8 va[DT];
+      bf16x8 va[2 * DC];                      // keys 16 j + 8 h .. of channel tile dt: 2 dt + j
       // (half of the values' operands when half of the keys' have been used, the rest behind them: there are no registers for both)
       auto read_values = [&](int from, int upto) {
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-          if (dt >= from && dt < upto) va[dt] = *reinterpret_cast<const bf16x8*>(lds_bytes + cur + rd_v + 256 * dt);
+        for (int i = 0; i < 2 * DC; ++i)
+          if (i >= from && i < upto) va[i] = *reinterpret_cast<const bf16x8*>(lds_bytes + cur + rd_v + 512 * (i % DC) + 2 * 512 * DC * (i / DC));
       };
-      uint32_t seen[CT];
-      float sv[CT][8];
-      float top[CT];
-      bool rises = false;
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        if constexpr (!FULL) {
-          const int first = t0 + 8 * g;
-          const int from = max(c.lo[ct] - first, 0), upto = min(c.hi[ct] - first, 7);
-          seen[ct] = ((there >> (g >> 1)) & 1) && upto >= from && from < 8 ? (2u << upto) - (1u << from) : 0u;
-        }
-        top[ct] = NONE;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          sv[ct][i] = st[ct][i >> 2][i & 3];
-          if constexpr (!FULL) sv[ct][i] = (seen[ct] >> i) & 1 ? sv[ct][i] : NONE;
-          top[ct] = fmaxf(top[ct], sv[ct][i]);
-        }
-        rises |= (top[ct] > 0.5f * NONE) & (top[ct] * sc > c.m[ct] + RESCALE_STEP);
+      // the lane's 16 keys: 8 h + i, and 16 + 8 h + i - 8 from i = 8 on
+      uint32_t seen = 0;
+      if constexpr (!FULL) {
+        const int from = max(lo - t0, 0), upto = min(hi - t0, 31);
+        const uint32_t range = upto >= from && from < 32 ? (uint32_t)((2ull << upto) - (1ull << from)) : 0u;
+        seen = (range & ((there & 1 ? 0xffffu : 0u) | (there & 2 ? 0xffff0000u : 0u))) >> (8 * h);
       }
-      if (__builtin_expect(__any(rises), 0)) {
+      auto sees = [&](int i) { return (seen >> (i < 8 ? i : i + 8)) & 1; };
+      float top = NONE;
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          const float t = max_of_column(top[ct]);
-          const float next = t > 0.5f * NONE ? t * sc : NONE;
-          if (next > c.m[ct] + RESCALE_STEP) {
-            const float f = __builtin_amdgcn_exp2f(c.m[ct] - next);
-            c.l[ct] *= f;
+      for (int i = 0; i < 16; ++i) {
+        if constexpr (!FULL) st[i] = sees(i) ? st[i] : NONE;
+        top = fmaxf(top, st[i]);
+      }
+      if (__builtin_expect(__any((top > 0.5f * NONE) & (top * sc > m + RESCALE_STEP)), 0)) {
+        const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+        const float t = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+        const float next = t > 0.5f * NONE ? t * sc : NONE;
+        // (a branch of the lanes, not of the wave: the sums are scaled in the registers that they are in)
+        if (next > m + RESCALE_STEP) {
+          const float f = __builtin_amdgcn_exp2f(m - next);
+          l *= f;
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
+          for (int dt = 0; dt < DC; ++dt)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) c.acc[ct][dt][i] *= f;
-            c.m[ct] = next;
-          }
+            for (int i = 0; i < 16; ++i) acc[dt][i] *= f;
+          m = next;
         }
       }
-      f32x4 sn[CT][2];
-      bf16x8 pb[CT];
-      float sum[CT], even[CT];
-      constexpr int NUMBERS = 8 * CT, SCORES = 2 * KS * CT;
+      f32x16 sn;
+      bf16x8 pb[2];
+      float sum = 0.f, even = 0.f;
 #pragma unroll
-      for (int i = 0; i < (NUMBERS > SCORES ? NUMBERS : SCORES); ++i) {
-        if (i == SCORES / 2) read_values(0, DT / 2);
-        if (i < SCORES) score(sn, i);
-        if (i < NUMBERS) {
-          const int ct = i % CT, e = i / CT;
-          float p = __builtin_amdgcn_exp2f(fmaf(sv[ct][e], sc, -c.m[ct]));
-          if constexpr (!FULL) p = (seen[ct] >> e) & 1 ? p : 0.f;      // while a column has seen no key, its reference point is NONE too
-          sum[ct] = e ? sum[ct] + p : p;
-          if (e & 1) { pb[ct][e - 1] = static_cast<bf16_t>(even[ct]); pb[ct][e] = static_cast<bf16_t>(p); }
-          else even[ct] = p;
-        }
+      for (int i = 0; i < 16; ++i) {
+        if (i == 8) read_values(0, DC);
+#pragma unroll
+        for (int ks = i * KS / 16; ks < (i + 1) * KS / 16; ++ks) sn = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[ks], q[ks], ks ? sn : zero, 0, 0, 0);
+        float p = __builtin_amdgcn_exp2f(fmaf(st[i], sc, -m));
+        if constexpr (!FULL) p = sees(i) ? p : 0.f;      // while a column has seen no key, its reference point is NONE too
+        sum = i ? sum + p : p;
+        if (i & 1) { pb[i >> 3][(i & 7) - 1] = static_cast<bf16_t>(even); pb[i >> 3][i & 7] = static_cast<bf16_t>(p); }
+        else even = p;
       }
       brought<4 * PIECES>();                  // block k + 2; k + 3 and k + 4 are still on their way
       read_raw(k + 2);
-      read_values(DT / 2, DT);
+      read_values(DC, 2 * DC);
+      l += sum;
       char *kbuf = lds_bytes + AT_K + (k & 1) * KBUF, *vbuf = lds_bytes + AT_V + to;
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) c.l[ct] += sum[ct];
+      for (int i = 0; i < 2 * DC; ++i) {
+        acc[i % DC] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[i], pb[i / DC], acc[i % DC], 0, 0, 0);
+        if constexpr (STEADY) {
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct) c.acc[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va[dt], pb[ct], c.acc[ct][dt], 0, 0, 0);
-          if constexpr (STEADY) {
-#pragma unroll
-            for (int j = dt * 4 / DT; j < (dt + 1) * 4 / DT; ++j) stage_store(std::true_type{}, j, k + 2, 3, kbuf, vbuf);
-          }
+          for (int j = i * 2 / DC; j < (i + 1) * 2 / DC; ++j) stage_store(std::true_type{}, j, k + 2, 3, kbuf, vbuf);
         }
+      }
       if constexpr (!STEADY) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) stage_store(std::false_type{}, j, k + 2, (hist >> 4) & 3, kbuf, vbuf);
@@ -688,8 +665,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
       pages = now; more_pages = later; codes = now_codes; more_codes = later_codes;
       hist = hist >> 2 | there_of(next) << 8;
       bring(next);
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) { st[ct][0] = sn[ct][0]; st[ct][1] = sn[ct][1]; }
+      st = sn;
       const uint32_t free = cur;
       cur = nxt; nxt = to; to = free;
       step_barrier();
@@ -707,38 +683,41 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
   }
   if (__builtin_expect(again, 0)) {
     // (zero times NaN: what such a block has added is of no use to the columns that do not see it)
-    for (int i = 0; i < 16 * CT; ++i) {
-      const int col = col0 + wave * CT * 16 + i;
-      if (col >= q_len * a.G) break;
-      const int tok = col / a.G;
-      one_column(a, table, q0 + tok, kvh, kvh * a.G + col - tok * a.G, max(seg_lo, first_seen(a, max(start + tok, 0))), min(seg_hi, start + tok + 1), seg, lane);
+    for (int i = 0; i < 32; ++i) {
+      const int c = col0 + 32 * wave + i;
+      if (c >= q_len * a.G) break;
+      const int t = c / a.G;
+      one_column(a, table, q0 + t, kvh, kvh * a.G + c - t * a.G, max(seg_lo, first_seen(a, max(start + t, 0))), min(seg_hi, start + t + 1), seg, lane);
     }
     return;
   }
+  const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+  l = __uint_as_float(both[0]) + __uint_as_float(both[1]);
+  if (!valid) return;
+  // the lane's channels: 32 dt + 8 i + 4 h .. + 3
+  if (a.num_parts > 1) {
+    const int64_t at = (row * a.Hq + head) * a.num_parts + seg;
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    const float l = sum_of_column(c.l[ct]);
-    const int col = col0 + (wave * CT + ct) * 16 + n;
-    if (col >= q_len * a.G) continue;
-    const int tok = col / a.G, head = kvh * a.G + col - tok * a.G;
-    const int64_t row = q0 + tok;
-    if (a.num_parts > 1) {
-      const int64_t at = (row * a.Hq + head) * a.num_parts + seg;
+    for (int dt = 0; dt < DC; ++dt)
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(a.part_o + at * HD + 16 * dt + 4 * g) = c.acc[ct][dt];
-      if (g == 0) { a.part_ml[2 * at] = c.m[ct]; a.part_ml[2 * at + 1] = l; }
-      continue;
-    }
-    const float inv = inverse(with_sink(a, head, c.m[ct], l));
-    bf16_t* o = a.out + row * a.out_stride + (int64_t)head * HD + 4 * g;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      bf16x4 r;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) r[i] = static_cast<bf16_t>(c.acc[ct][dt][i] * inv);
-      *reinterpret_cast<bf16x4*>(o + 16 * dt) = r;
-    }
+      for (int i = 0; i < 4; ++i)
+        if (32 * dt + 8 * i < HD)
+          *reinterpret_cast<f32x4*>(a.part_o + at * HD + 32 * dt + 8 * i + 4 * h) = f32x4{acc[dt][4 * i], acc[dt][4 * i + 1], acc[dt][4 * i + 2], acc[dt][4 * i + 3]};
+    if (h == 0) { a.part_ml[2 * at] = m; a.part_ml[2 * at + 1] = l; }
+    return;
   }
+  const float inv = inverse(with_sink(a, head, m, l));
+  bf16_t* o = a.out + row * a.out_stride + (int64_t)head * HD + 4 * h;
+#pragma unroll
+  for (int dt = 0; dt < DC; ++dt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (32 * dt + 8 * i < HD) {
+        bf16x4 r;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = static_cast<bf16_t>(acc[dt][4 * i + e] * inv);
+        *reinterpret_cast<bf16x4*>(o + 32 * dt + 8 * i) = r;
+      }
 }
 
 // Joins the partitions of a (row, head): out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p. A wave to a (row, head); partitions
@@ -835,32 +814,19 @@ extern "C" int me_attn8_decode(const void* q, int64_t q_stride, void* out, int64
 extern "C" int me_attn8_prompt(const void* q, int64_t q_stride, void* out, int64_t out_stride, const void* k, const void* v,
                                const void* k_powers, const void* v_powers, int64_t num_pages, const int32_t* tables, int table_stride,
                                int table_cols, const int32_t* contexts, const int32_t* cu, int64_t rows, int num_seqs, int Hq, int Hkv,
-                               int page, float scale, int window, int chunk, int col_tiles, int part_keys, int num_parts, float* scratch,
+                               int page, float scale, int window, int chunk, int part_keys, int num_parts, float* scratch,
                                const float* sinks, hipStream_t stream) {
   Attn8Args a;
   if (int rc = fill(a, q, q_stride, out, out_stride, k, v, k_powers, v_powers, num_pages, tables, table_stride, table_cols, contexts,
                     num_seqs, Hq, Hkv, page, scale, window, chunk, part_keys, num_parts, scratch, rows, sinks)) return rc;
   a.cu = cu;
-  ME_CHECK(col_tiles == 1 || (col_tiles == 2 && HD <= 128), "attention_e4m3: %d column tiles per wave", col_tiles);
-  const int64_t tiles = rows * a.G / (64 * col_tiles) + num_seqs;
+  const int64_t tiles = rows * a.G / COLS + num_seqs;
   ME_CHECK(rows >= 1 && rows * a.G < (1ll << 30) && tiles * Hkv < (1ll << 31), "attention_e4m3: too many tokens for one launch");
-  const dim3 grid((unsigned)(tiles * Hkv), num_parts);
-  constexpr int lds = LDS_BYTES;
-#define PROMPT(CT)                                                                                                                   \
-  do {                                                                                                                               \
-    if (lds > 64 * 1024) {                                                                                                           \
-      hipError_t e = hipFuncSetAttribute((const void*)attn8_prompt_kernel<CT>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);     \
-      ME_CHECK(e == hipSuccess, "attention_e4m3: %d bytes of shared memory: %s", lds, hipGetErrorString(e));                         \
-    }                                                                                                                                \
-    attn8_prompt_kernel<CT><<<grid, 256, lds, stream>>>(a, (int)tiles);                                                              \
-  } while (0)
-  if constexpr (HD <= 128) {
-    if (col_tiles == 2) PROMPT(2);
-    else PROMPT(1);
-  } else {
-    PROMPT(1);
+  if (LDS_BYTES > 64 * 1024) {
+    hipError_t e = hipFuncSetAttribute((const void*)attn8_prompt_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS_BYTES);
+    ME_CHECK(e == hipSuccess, "attention_e4m3: %d bytes of shared memory: %s", LDS_BYTES, hipGetErrorString(e));
   }
-#undef PROMPT
+  attn8_prompt_kernel<<<dim3((unsigned)(tiles * Hkv), num_parts), 256, LDS_BYTES, stream>>>(a, (int)tiles);
   ME_LAUNCH_CHECK();
   return join(a, rows, stream);
 }

@@ -137,7 +137,7 @@ _ATTN_PROTOS = {
 
 _ATTN_E4M3_PROTOS = {
     "me_attn8_decode": [P, L, P, L, P, P, P, P, L, P, I, I, P, I, I, I, I, F, I, I, I, I, P, P, P],
-    "me_attn8_prompt": [P, L, P, L, P, P, P, P, L, P, I, I, P, P, L, I, I, I, I, F, I, I, I, I, I, P, P, P],
+    "me_attn8_prompt": [P, L, P, L, P, P, P, P, L, P, I, I, P, P, L, I, I, I, I, F, I, I, I, I, P, P, P],
 }
 
 _core: _Lib | None = None
@@ -761,11 +761,11 @@ class HipBackend:
                      _ptr(scratch), _ptr(sinks), _stream())
         if T > num_decodes:
             Tp = T - num_decodes
-            tiles, part, parts = prompt_partitions_e4m3(Tp, B - num_decodes, Hq, Hkv, D, max_prefill_context or block_tables.shape[1] * page, span)
+            part, parts = prompt_partitions_e4m3(Tp, B - num_decodes, Hq, Hkv, D, max_prefill_context or block_tables.shape[1] * page, span)
             scratch = torch.empty(Tp * Hq * parts * (D + 2), dtype=torch.float32, device=q.device) if parts > 1 else None
             lib.call("me_attn8_prompt", q.data_ptr() + num_decodes * rows * 2, rows, out.data_ptr() + num_decodes * Hq * D * 2, Hq * D, *pools,
                      block_tables.data_ptr() + num_decodes * tables[0] * 4, *tables, context_lens.data_ptr() + num_decodes * 4,
-                     prefill_cu.data_ptr(), Tp, B - num_decodes, Hq, Hkv, page, float(scale), int(window or 0), int(chunk or 0), tiles, part, parts,
+                     prefill_cu.data_ptr(), Tp, B - num_decodes, Hq, Hkv, page, float(scale), int(window or 0), int(chunk or 0), part, parts,
                      _ptr(scratch), _ptr(sinks), _stream())
         return out
 
@@ -1632,16 +1632,15 @@ def decode_partitions_e4m3(num_seqs: int, Hq: int, Hkv: int, max_context: int, s
 
 
 def prompt_partitions_e4m3(tokens: int, num_seqs: int, Hq: int, Hkv: int, D: int, max_context: int, span: int = 0) -> tuple:
-    """(column tiles of a wave, keys per partition, partitions) of a launch of prompt portions over an 8-bit cache."""
+    """(keys per partition, partitions) of a launch of prompt portions over an 8-bit cache, in tiles of 128 (token, head) pairs."""
     G = Hq // Hkv
-    tiles = 2 if D <= 128 and tokens * G > 64 * num_seqs else 1
-    keys = max(1, min(max_context, span + 64 * tiles // G + 64) if span else max_context)
-    groups = (tokens * G // (64 * tiles) + 1) * Hkv
+    keys = max(1, min(max_context, span + 128 // G + 64) if span else max_context)
+    groups = (tokens * G // 128 + 1) * Hkv
     parts = max(1, min(-(-512 // groups), keys // 512))
     if parts == 1:
-        return tiles, 0, 1
+        return 0, 1
     part = -(-keys // (parts * 64)) * 64
-    return tiles, part, -(-keys // part)
+    return part, -(-keys // part)
 
 
 def prefill_col_tiles(max_context: int, window: int, num_tokens: int, Hq: int, D: int = 128) -> int:
