@@ -326,8 +326,8 @@ __global__ void __launch_bounds__(256) attn8_decode_kernel(Attn8Args a) {
 // two lanes (l and l ^ 32). The workgroup walks the keys that its columns see in blocks of 32 with v_mfma_f32_32x32x16_bf16 (half as many
 // instructions as tiles of 16 x 16 take, and one column's state to a lane instead of two). Row r of a tile of scores stands for the key whose bits 2
 // and 3 are exchanged: lane l then holds keys 8 h .. 8 h + 7 and 16 + 8 h .. of its column (h = l / 32), the values' operand as it is.
-// A block's bytes go to LDS by themselves (global_load_lds_dwordx4), five blocks ahead, and are turned into bfloat16 once, two blocks
-// ahead, from which every wave reads its operands (each wave all conversions for itself would be a third of its vector instructions; bytes
+// A block's bytes go to LDS by themselves (global_load_lds_dwordx4), five and six blocks ahead, and are turned into bfloat16 once, two and
+// three blocks ahead, from which every wave reads its operands (each wave all conversions for itself would be a third of its vector instructions; bytes
 // held in registers could be asked for one step ahead only, less than a trip to memory). What a wave brings of a block lies in one page
 // under one power, so pages, powers and addresses are scalars, and a lane turns into bfloat16 what it has brought itself.
 //   keys    [pieces of 8 channels][32 rows] of 16 bytes: a read of 16 bytes a lane is worked off for lanes 0-3, 12-15 and 20-27 together,
@@ -335,7 +335,9 @@ __global__ void __launch_bounds__(256) attn8_decode_kernel(Attn8Args a) {
 //           change places in every second pair of pieces (row ^ 4), which spreads the writes over all banks and leaves the reads as they are.
 //   values  [8 keys][channel] of 16 bytes.
 // Step k of the walk is a pipeline: beside the numbers of block k's softmax the products of block k + 1's scores, beside the products of
-// its values block k + 2's conversion. One barrier a step. LDS: bytes of four blocks, keys of two, values of three.
+// its values the conversion of block k + 2's values and block k + 3's keys and the reads of block k + 2's keys (read in front of their
+// products instead, behind the barrier, every step began with a wait for LDS). One barrier a step. LDS: bytes of four blocks, keys of two,
+// values of three.
 // Grid (tiles x key heads, segments): surplus tiles (the grid is made for the most there can be) exit.
 // =====================================================================================
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -487,80 +489,69 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
     const uint8_t* k_head = a.k + (((int64_t)kvh << a.page_shift) + 8 * part) * HD;
     const uint8_t* v_head = a.v + (((int64_t)kvh * HD + part * (HD / 2)) << a.page_shift);
     const uint32_t k_lane = (lane & 7) * HD + (lane >> 3) * 16, v_lane = (uint32_t)lane << a.page_shift;
-    auto bring = [&](int k) {
-      const int off = (seg_lo + PB * k + 16 * group) & page_mask;
-      const uint64_t at = (uint64_t)(uint32_t)max(__builtin_amdgcn_readlane(pages, (2 * k + group) & 63), 0) * page_bytes;
-      const uint32_t slot = lds0 + AT_RAW + (k & 3) * (2 * RAW) + 1024 * PIECES * wave;
+    const uint32_t my_slot = lds0 + AT_RAW + 1024 * PIECES * wave;
+    auto offset_of = [&](int k) { return (seg_lo + PB * k + 16 * group) & page_mask; };
+    auto page_of = [&](int k) { return (uint64_t)(uint32_t)max(__builtin_amdgcn_readlane(pages, (2 * k + group) & 63), 0) * page_bytes; };
+    auto bring_keys = [&](int k, uint64_t page) {
 #pragma unroll
       for (int i = 0; i < PIECES; ++i)
-        if (HD % 128 == 0 || lane + 64 * i < HD / 2) {
-          bring16(k_head + at + off * HD + 128 * i, k_lane, slot + 1024 * i);
-          bring16(v_head + at + off + ((int64_t)(64 * i) << a.page_shift), v_lane, slot + RAW + 1024 * i);
-        }
+        if (HD % 128 == 0 || lane + 64 * i < HD / 2) bring16(k_head + page + offset_of(k) * HD + 128 * i, k_lane, my_slot + (k & 3) * (2 * RAW) + 1024 * i);
+    };
+    auto bring_values = [&](int k, uint64_t page) {
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i)
+        if (HD % 128 == 0 || lane + 64 * i < HD / 2)
+          bring16(v_head + page + offset_of(k) + ((int64_t)(64 * i) << a.page_shift), v_lane, my_slot + (k & 3) * (2 * RAW) + RAW + 1024 * i);
     };
     u32x4v raw_k[PIECES], raw_v[PIECES];
-    auto read_raw = [&](int k) {
+    auto read_raw_keys = [&](int k) {
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) raw_k[i] = *reinterpret_cast<const u32x4v*>(lds_bytes + AT_RAW + (k & 3) * (2 * RAW) + mine + 1024 * i);
+    };
+    auto read_raw_values = [&](int k) {
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) raw_v[i] = *reinterpret_cast<const u32x4v*>(lds_bytes + AT_RAW + (k & 3) * (2 * RAW) + RAW + mine + 1024 * i);
+    };
+    // Half j of a block's keys as bfloat16. Of the wave's 8 keys 16 group + 8 part + r: row 16 group + 8 (r / 4) + 4 part + r % 4; channels
+    // 16 c + 8 j ..: piece 2 c + j.
+    auto store_keys = [&](int j, uint32_t code, char* kbuf) {
+      const float power = __uint_as_float(code & 0x7f800000u);
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
-        const char* slot = lds_bytes + AT_RAW + (k & 3) * (2 * RAW) + mine + 1024 * i;
-        raw_k[i] = *reinterpret_cast<const u32x4v*>(slot);
-        raw_v[i] = *reinterpret_cast<const u32x4v*>(slot + RAW);
+        const int r = lane & 7, c = (lane >> 3) + 8 * i;
+        char* to = kbuf + (2 * c * PB + ((16 * group + 8 * (r >> 2) + 4 * part + (r & 3)) ^ (4 * ((c >> 1) & 1)))) * 16;
+        if (HD % 128 == 0 || 16 * c < HD) *reinterpret_cast<bf16x8*>(to + 16 * PB * j) = operand(raw_k[i][2 * j], raw_k[i][2 * j + 1], power);
       }
     };
-    // Part j of 4 of a block as bfloat16. Values of keys in front of tile_lo, or from L on, or in no page become zeros; a NaN among the
-    // others is reported. WHOLE: every column of the tile sees all of the block, and it lies in pages.
-    auto stage_store = [&](auto whole_tag, int j, int k, uint32_t there, char* kbuf, char* vbuf) {
+    // Half j of block k's values. Keys in front of tile_lo, or from L on, or in no page become zeros; a NaN among the others is reported.
+    // WHOLE: every column of the tile sees all of the block, and it lies in pages.
+    auto store_values = [&](auto whole_tag, int j, int k, uint32_t code, uint32_t there, char* vbuf) {
       constexpr bool WHOLE = decltype(whole_tag)::value;
-      const int first = seg_lo + PB * k + 16 * group;
-      const uint32_t code = __builtin_amdgcn_readlane(codes, (2 * k + group) & 63);
+      const float power = __uint_as_float((code << 8) & 0x7f800000u);
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
-        if (j < 2) {
-          // of the wave's 8 keys 16 group + 8 part + r: row 16 group + 8 (r / 4) + 4 part + r % 4; channels 16 c + 8 j ..: piece 2 c + j
-          const float kp = __uint_as_float(code & 0x7f800000u);
-          const int r = lane & 7, c = (lane >> 3) + 8 * i;
-          char* kd = kbuf + (2 * c * PB + ((16 * group + 8 * (r >> 2) + 4 * part + (r & 3)) ^ (4 * ((c >> 1) & 1)))) * 16;
-          if (HD % 128 == 0 || 16 * c < HD) *reinterpret_cast<bf16x8*>(kd + 16 * PB * j) = operand(raw_k[i][2 * j], raw_k[i][2 * j + 1], kp);
-        } else {
-          const int half = j - 2, p = lane + 64 * i;
-          const float vp = __uint_as_float((code << 8) & 0x7f800000u);
-          uint32_t w0 = raw_v[i][2 * half], w1 = raw_v[i][2 * half + 1];
+        const int p = lane + 64 * i;
+        uint32_t w0 = raw_v[i][2 * j], w1 = raw_v[i][2 * j + 1];
+        if constexpr (!WHOLE) {
+          const int first = seg_lo + PB * k + 16 * group;
+          if (!((there >> group) & 1) || first < tile_lo || first + 16 > L) {
+            const int from = ((there >> group) & 1) ? tile_lo - first - 8 * j : 8, to = L - first - 8 * j;
+            const uint64_t upto = to >= 8 ? ~0ull : to <= 0 ? 0ull : (1ull << (8 * to)) - 1, below = from >= 8 ? ~0ull : from <= 0 ? 0ull : (1ull << (8 * from)) - 1;
+            const uint64_t keep = upto & ~below;
+            w0 &= (uint32_t)keep; w1 &= (uint32_t)(keep >> 32);
+          }
+        }
+        if (HD % 128 == 0 || p < HD / 2) {
           if constexpr (!WHOLE) {
-            if (!((there >> group) & 1) || first < tile_lo || first + 16 > L) {
-              const int from = ((there >> group) & 1) ? tile_lo - first - 8 * half : 8, to = L - first - 8 * half;
-              const uint64_t upto = to >= 8 ? ~0ull : to <= 0 ? 0ull : (1ull << (8 * to)) - 1, below = from >= 8 ? ~0ull : from <= 0 ? 0ull : (1ull << (8 * from)) - 1;
-              const uint64_t keep = upto & ~below;
-              w0 &= (uint32_t)keep; w1 &= (uint32_t)(keep >> 32);
-            }
+            // all seven lower bits of a byte
+            const uint32_t nan = (((w0 & 0x7f7f7f7fu) + 0x01010101u) | ((w1 & 0x7f7f7f7fu) + 0x01010101u)) & 0x80808080u;
+            if (__builtin_expect(nan != 0, 0)) *nan_flag = 1;
           }
-          if (HD % 128 == 0 || p < HD / 2) {
-            if constexpr (!WHOLE) {
-              // all seven lower bits of a byte
-              const uint32_t nan = (((w0 & 0x7f7f7f7fu) + 0x01010101u) | ((w1 & 0x7f7f7f7fu) + 0x01010101u)) & 0x80808080u;
-              if (__builtin_expect(nan != 0, 0)) *nan_flag = 1;
-            }
-            *reinterpret_cast<bf16x8*>(vbuf + ((2 * group + half) * (32 * DC) + part * (HD / 2) + p) * 16) = operand(w0, w1, vp);
-          }
+          *reinterpret_cast<bf16x8*>(vbuf + ((2 * group + j) * (32 * DC) + part * (HD / 2) + p) * 16) = operand(w0, w1, power);
         }
       }
     };
-
-    // blocks 0 and 1 as bfloat16, 2 to 4 on their way
-    uint32_t hist = 0;                        // two bits for every block from the current one on: its groups in pages
-#pragma unroll
-    for (int k = 0; k < 4; ++k) bring(k);
-#pragma unroll
-    for (int k = 0; k < 5; ++k) hist |= there_of(k) << (2 * k);
-    step_barrier();                           // (the flags and the zeros)
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      if (k == 0) brought<6 * PIECES>(); else brought<4 * PIECES>();
-      read_raw(k);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) stage_store(std::false_type{}, j, k, there_of(k), lds_bytes + AT_K + k * KBUF, lds_bytes + AT_V + k * VBUF);
-    }
-    step_barrier();                           // (the bytes of block 0 have been read)
-    bring(4);
+    auto code_of_block = [&](int k) { return (uint32_t)__builtin_amdgcn_readlane(codes, (2 * k + group) & 63); };
 
     const float sc = a.scale * LOG2E;
     const uint32_t rd_v = AT_V + (32 * DC * h + n) * 16;
@@ -573,10 +564,39 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
     };
     const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     f32x16 st;                                // the scores of the block whose softmax comes next
+
+    // What the first step finds: block 0's scores, block 1's keys in registers and block 2's in LDS, the values of 0 and 1 in LDS, and on their
+    // way, in this order, the keys and values of (3, 2), (4, 3), (5, 4).
+    uint32_t hist = 0;                        // two bits for every block from the current one on: its groups in pages
+#pragma unroll
+    for (int k = 0; k < 6; ++k) hist |= there_of(k) << (2 * k);
+    bring_keys(0, page_of(0)); bring_keys(1, page_of(1)); bring_values(0, page_of(0)); bring_values(1, page_of(1)); bring_keys(2, page_of(2));
+    bring_keys(3, page_of(3)); bring_values(2, page_of(2)); bring_values(3, page_of(3));
+    step_barrier();                           // (the flag)
+    brought<3 * PIECES>();
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      read_raw_keys(k); read_raw_values(k);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        store_keys(j, code_of_block(k), lds_bytes + AT_K + k * KBUF);
+        store_values(std::false_type{}, j, k, code_of_block(k), there_of(k), lds_bytes + AT_V + k * VBUF);
+      }
+    }
+    read_raw_keys(2);
+    step_barrier();
+    bring_keys(4, page_of(4)); bring_keys(5, page_of(5)); bring_values(4, page_of(4));
     read_keys(0);
-    step_barrier();                           // (the first step writes block 2 over block 0's keys)
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[ks], q[ks], ks ? st : zero, 0, 0, 0);
+    read_keys(KBUF);
+    step_barrier();
+#pragma unroll
+    for (int j = 0; j < 2; ++j) store_keys(j, code_of_block(2), lds_bytes + AT_K);
+    step_barrier();
+    uint32_t code_v = code_of_block(2);       // of the block whose values are turned into bfloat16 next
+    uint64_t page_v = page_of(5);             // of the block whose values are asked for next
 
     uint32_t cur = 0, nxt = VBUF, to = 2 * VBUF;        // the values of blocks k, k + 1, k + 2
     // STEADY: every column of the wave sees every key of block k, every one of the tile those of block k + 2, and both lie in pages; such a
@@ -585,12 +605,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
       constexpr bool STEADY = decltype(steady_tag)::value, FULL = STEADY;
       const int t0 = seg_lo + PB * k;
       const uint32_t there = hist & 3;
-      read_keys(((k + 1) & 1) * KBUF);         // (behind the last block: what lies there is not used)
-      __builtin_amdgcn_sched_barrier(0);
-      bf16x8 va[2 * DC];                      // keys 16 j + 8 h .. of channel tile dt: 2 dt + j
-      // (half of the values' operands when half of the keys' have been used, the rest behind them: there are no registers for both)
+      brought<4 * PIECES>();                  // keys of block k + 3, values of k + 2; the two steps' after them are still on their way
+      read_raw_keys(k + 3);
+      read_raw_values(k + 2);
+      const uint32_t code_k = code_of_block(k + 3);
+      bf16x8 va[2 * DC];                      // keys 16 j + 8 h .. of channel tile dt: DC j + dt
       auto read_values = [&](int from, int upto) {
-        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < 2 * DC; ++i)
           if (i >= from && i < upto) va[i] = *reinterpret_cast<const bf16x8*>(lds_bytes + cur + rd_v + 512 * (i % DC) + 2 * 512 * DC * (i / DC));
@@ -629,7 +649,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
       float sum = 0.f, even = 0.f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        if (i == 8) read_values(0, DC);
+        // the values' operands take the registers of the keys' that have been used
+        if (i == 8) { __builtin_amdgcn_sched_barrier(0); read_values(0, DC); }
+        if (i == 12) { __builtin_amdgcn_sched_barrier(0); read_values(DC, 2 * DC); }
 #pragma unroll
         for (int ks = i * KS / 16; ks < (i + 1) * KS / 16; ++ks) sn = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[ks], q[ks], ks ? sn : zero, 0, 0, 0);
         float p = __builtin_amdgcn_exp2f(fmaf(st[i], sc, -m));
@@ -638,33 +660,41 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
         if (i & 1) { pb[i >> 3][(i & 7) - 1] = static_cast<bf16_t>(even); pb[i >> 3][i & 7] = static_cast<bf16_t>(p); }
         else even = p;
       }
-      brought<4 * PIECES>();                  // block k + 2; k + 3 and k + 4 are still on their way
-      read_raw(k + 2);
-      read_values(DC, 2 * DC);
+      __builtin_amdgcn_sched_barrier(0);
       l += sum;
-      char *kbuf = lds_bytes + AT_K + (k & 1) * KBUF, *vbuf = lds_bytes + AT_V + to;
+      char *kbuf = lds_bytes + AT_K + ((k + 1) & 1) * KBUF, *vbuf = lds_bytes + AT_V + to;
 #pragma unroll
       for (int i = 0; i < 2 * DC; ++i) {
+        if (i == DC) { __builtin_amdgcn_sched_barrier(0); read_keys((k & 1) * KBUF); }      // block k + 2's, where half of the values' have been used
         acc[i % DC] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[i], pb[i / DC], acc[i % DC], 0, 0, 0);
         if constexpr (STEADY) {
 #pragma unroll
-          for (int j = i * 2 / DC; j < (i + 1) * 2 / DC; ++j) stage_store(std::true_type{}, j, k + 2, 3, kbuf, vbuf);
+          for (int j = i * 2 / DC; j < (i + 1) * 2 / DC; ++j) {
+            if (j < 2) store_keys(j, code_k, kbuf);
+            else store_values(std::true_type{}, j - 2, k + 2, code_v, 3, vbuf);
+          }
         }
       }
       if constexpr (!STEADY) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) stage_store(std::false_type{}, j, k + 2, (hist >> 4) & 3, kbuf, vbuf);
+        for (int j = 0; j < 2; ++j) {
+          store_keys(j, code_k, kbuf);
+          store_values(std::false_type{}, j, k + 2, code_v, (hist >> 4) & 3, vbuf);
+        }
       }
       // (what is held for 32 blocks is stored whether it has changed or not: a store in each branch would put it into scratch memory)
-      const int next = k + 5, t_next = seg_lo + PB * next;
+      const int next = k + 6, t_next = seg_lo + PB * next;
       int now = pages, later = more_pages;
       uint32_t now_codes = codes, later_codes = more_codes;
       if (__builtin_expect((next & 31) == 31, 0)) { asm volatile("" ::: "memory"); later = ask_pages(t_next + PB); }
       if (__builtin_expect((next & 31) == 0, 0)) { asm volatile("" ::: "memory"); now = settle_pages(t_next, later); later_codes = ask_codes(t_next, now); held = __ballot(now >= 0); }
-      if (__builtin_expect((next & 31) == 2, 0)) now_codes = later_codes;          // the next step turns block k + 3 into bfloat16, the first of its 32
+      if (__builtin_expect((next & 31) == 2, 0)) now_codes = later_codes;          // the next step turns block k + 4's keys into bfloat16, the first of its 32
       pages = now; more_pages = later; codes = now_codes; more_codes = later_codes;
-      hist = hist >> 2 | there_of(next) << 8;
-      bring(next);
+      hist = hist >> 2 | there_of(next) << 10;
+      const uint64_t page_k = page_of(next);
+      bring_keys(next, page_k);
+      bring_values(next - 1, page_v);
+      page_v = page_k; code_v = code_k;
       st = sn;
       const uint32_t free = cur;
       cur = nxt; nxt = to; to = free;
