@@ -2,6 +2,7 @@
 
 What a page holds is the mixer's business (`CacheNeed.tensors`); attention's layout is
     K [num_pages, Hkv, page, D]   V [num_pages, Hkv, D, page]
+and in 8 bits the same of e4m3 numbers beside a byte for every 16 tokens and head
 (not the reference's [blocks, block, Hkv, D], engine/model_runner.py:9-17: chosen for the matrix-core
 attention kernels). A group's pool stacks the calls that own pages in it: [calls, num_pages + 1, ...].
 One page more than the manager hands out, and one state row more than it has slots: spares that belong
@@ -16,7 +17,7 @@ import torch
 from ..kernels import ops
 from ..parts.base import CacheView
 
-_DTYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "int32": torch.int32}
+_DTYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "int32": torch.int32, "e4m3": torch.float8_e4m3fn, "uint8": torch.uint8}
 
 
 def _dtype_of(name: str, compute: torch.dtype) -> torch.dtype:

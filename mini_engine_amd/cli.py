@@ -47,6 +47,7 @@ def main(argv=None) -> int:
     p.add_argument("--max-model-len", type=int, default=2048)
     p.add_argument("--max-num-seqs", type=int, default=256)
     p.add_argument("--block-size", type=int, default=16, help="kvcache_block_size")
+    p.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "e4m3"], help="e4m3: keys and values in 8 bits")
     p.add_argument("--policy", default="fcfs", choices=["fcfs", "priority"])
     p.add_argument("--max-prompt", type=int, default=1024)
     p.add_argument("--max-output", type=int, default=1024)
@@ -104,7 +105,7 @@ def main(argv=None) -> int:
     llm = LLM(path, max_num_seqs=args.max_num_seqs, max_model_len=args.max_model_len, max_num_batched_tokens=args.budget,
               enable_chunked_prefill=bool(args.chunked), long_prefill_token_threshold=args.threshold, dtype=args.dtype,
               seed=args.seed, kvcache_block_size=args.block_size, scheduling_policy=args.policy, device=args.device,
-              num_kvcache_blocks=args.num_kv_blocks)
+              num_kvcache_blocks=args.num_kv_blocks, kv_cache_dtype=args.kv_cache_dtype)
     vocab = llm.model.embedding.vocab_size
     if vocab_cap is not None and vocab <= vocab_cap:
         prompt_token_ids = [[t % vocab for t in ids] for ids in prompt_token_ids]
@@ -127,7 +128,7 @@ def main(argv=None) -> int:
     total = sum(len(r["token_ids"]) for r in results)
     row = {
         "engine": "mini_engine_amd", "label": args.label, "gpu": torch.cuda.get_device_name(0) if args.device.startswith("cuda") else args.device, "torch": torch.__version__,
-        "model": args.random_weights or path, "dtype": args.dtype, "num_seqs": N,
+        "model": args.random_weights or path, "dtype": args.dtype, "kv_cache_dtype": args.kv_cache_dtype, "num_seqs": N,
         "input_tokens": sum(len(x) for x in prompt_token_ids), "output_tokens": total, "time_s": round(t, 2),
         "throughput_tok_s": round(total / t, 1), "chunked": bool(args.chunked), "budget": args.budget,
         "threshold": args.threshold, "preemptions": llm.scheduler.num_preemptions,

@@ -187,6 +187,7 @@ def main(argv=None) -> int:
     p.add_argument("--out", default="results/latency.jsonl")
     p.add_argument("--label", default="")
     p.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    p.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "e4m3"], help="e4m3: keys and values in 8 bits")
     p.add_argument("--seed", type=int, default=0, help="seed of the sampler's noise and of random weights")
     p.add_argument("--max-model-len", type=int, default=8192)
     p.add_argument("--max-num-seqs", type=int, default=128)
@@ -213,7 +214,7 @@ def main(argv=None) -> int:
     path = os.path.expanduser(path)
 
     engine = LLM(path, max_num_seqs=args.max_num_seqs, max_model_len=args.max_model_len,
-                 max_num_batched_tokens=ENGINE_BUDGET, dtype=args.dtype, seed=args.seed)
+                 max_num_batched_tokens=ENGINE_BUDGET, dtype=args.dtype, seed=args.seed, kv_cache_dtype=args.kv_cache_dtype)
     vocab = engine.model.embedding.vocab_size
     params_of = lambda a: SamplingParams(temperature=0.6, ignore_eos=True, max_tokens=a.max_tokens)
     settings = [Setting.parse(name) for name in args.configs.split(",") if name]
@@ -228,7 +229,7 @@ def main(argv=None) -> int:
     sweep(engine, [Setting.parse("c2048")], [20.0], workload, 20, params_of, lambda *ignored: None)
 
     os.makedirs(os.path.dirname(args.out) or ".", exist_ok=True)
-    about = {"model": args.random_weights or path, "dtype": args.dtype, "gpu": torch.cuda.get_device_name(0),
+    about = {"model": args.random_weights or path, "dtype": args.dtype, "kv_cache_dtype": args.kv_cache_dtype, "gpu": torch.cuda.get_device_name(0),
              "torch": torch.__version__}
 
     def emit(rate, setting, figures):

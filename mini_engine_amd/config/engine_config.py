@@ -2,7 +2,8 @@
 
 Added beside the reference's fields: ``dtype`` (bfloat16 or a true float32 path),
 ``seed`` (sampling noise is a function of seed, request and output index),
-``enable_prefix_caching``, ``use_graphs``, ``run_ahead`` and ``random_weights``; ``num_kvcache_blocks`` may be given
+``enable_prefix_caching``, ``use_graphs``, ``run_ahead``, ``random_weights`` and ``kv_cache_dtype`` ("auto": the
+compute type; "e4m3": 8 bits under a power of two per 16 tokens and head); ``num_kvcache_blocks`` may be given
 (the reference always sizes the pool itself, ``engine/model_runner.py:46-48``).
 """
 from __future__ import annotations
@@ -13,6 +14,7 @@ from dataclasses import dataclass, field, fields
 from .model_config import ConfigError, load_model_config
 
 DTYPES = ("bfloat16", "float32")
+KV_CACHE_DTYPES = ("auto", "e4m3")
 
 
 @dataclass
@@ -34,6 +36,7 @@ class EngineConfig:
     use_graphs: bool = True
     run_ahead: bool = True                # launch the next plain decode step before this one's tokens are fetched
     random_weights: int | None = None     # a seed: the folder needs only config.json, weights are drawn on the device
+    kv_cache_dtype: str = "auto"          # "e4m3": keys and values in 8 bits, half the bytes and twice the tokens of bfloat16
     model_config: object = field(default=None, repr=False)
 
     @classmethod
@@ -53,6 +56,13 @@ class EngineConfig:
             self.dtype = "float32"
         if self.dtype not in DTYPES:
             raise ConfigError(f"dtype must be one of {DTYPES}, got {self.dtype!r}")
+        if self.kv_cache_dtype not in KV_CACHE_DTYPES:
+            raise ConfigError(f"kv_cache_dtype must be one of {KV_CACHE_DTYPES}, got {self.kv_cache_dtype!r}")
+        if self.kv_cache_dtype == "e4m3":
+            if self.dtype != "bfloat16":
+                raise ConfigError("keys and values in 8 bits are for bfloat16 models")
+            if self.kvcache_block_size < 16 or self.kvcache_block_size & (self.kvcache_block_size - 1):
+                raise ConfigError(f"keys and values in 8 bits take a kvcache_block_size of a power of two from 16 on, got {self.kvcache_block_size}")
         if self.max_num_batched_tokens < self.max_num_seqs:
             raise ConfigError("max_num_batched_tokens must be >= max_num_seqs "
                               "(every running request must be able to decode in one step)")

@@ -11,6 +11,7 @@ import torch
 from ..cache.manager import CacheManager
 from ..cache.pool import page_bytes
 from ..config.engine_config import EngineConfig
+from ..config.model_config import ConfigError
 from ..sampling.sampler import Sampler
 from ..sampling.sampling_params import SamplingParams
 from ..weights.loader import load_model
@@ -75,6 +76,11 @@ class LLMEngine:
         self.dtype = _DTYPES[config.dtype]
         self.model = load_model(config.model, self.device, self.dtype, config.max_model_len, config.model_config,
                                 random_weights=config.random_weights)
+        if config.kv_cache_dtype != "auto":
+            try:
+                self.model.hold_keys_and_values_in(config.kv_cache_dtype)
+            except ValueError as e:
+                raise ConfigError(f"kv_cache_dtype {config.kv_cache_dtype!r}: {e}") from None
         plan = self.model.cache_plan()
         self._state_slots = config.max_num_seqs if any(s is not None for s in plan.state_needs) else 0
         self.reserved_bytes = 0

@@ -60,6 +60,19 @@ class DecoderModel(Part):
             if call.cache_of is not None and not 0 <= call.cache_of < i:
                 raise ValueError(f"run order entry {i} may only read the cache of an earlier entry, got {call.cache_of}")
 
+    def hold_keys_and_values_in(self, kind: str) -> None:
+        """`kind`: what the attention layers' pages hold, "compute" (the engine's data type) or "e4m3" (8 bits under a power of two per
+        16 tokens and head). Other mixers keep what they keep. Raises ValueError where a layer's attention has no such form, or where
+        no layer keeps keys and values. Before the cache is made."""
+        holders = [(i, part) for i, layer in enumerate(self.layers) for part in layer.parts() if hasattr(part, "hold_in")]
+        if kind != "compute" and not holders:
+            raise ValueError("no layer of this model keeps keys and values: there is nothing to hold in 8 bits")
+        for i, mixer in holders:
+            try:
+                mixer.hold_in(kind)
+            except ValueError as e:
+                raise ValueError(f"layer {i}: {e}") from None
+
     # -- what the cache has to provide ------------------------------------------------------
     def cache_plan(self) -> CachePlan:
         keys: dict = {}

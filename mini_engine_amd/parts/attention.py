@@ -173,12 +173,30 @@ class Attention(Mixer):
         if value_mix == "blend":
             self.add_param("vmix", ParamSpec((), init=_half, dtype="float32"))
         self.norm_eps = qk_norm_eps
+        self.pages_hold = "compute"
         if position is not None:
             self.add_child("position", position)
         else:
             self.position = None
 
+    def hold_in(self, kind: str) -> None:
+        """What the pages hold: "compute", the engine's data type, or "e4m3", 8 bits under a power of two per 16 tokens and head
+        (`ops.PagesE4M3`), which half of the bytes pays for with 4 significant bits. The kernels over such pages know no biases or
+        whole-projection norms, kept first keys, score caps or slopes."""
+        if kind not in ("compute", "e4m3"):
+            raise ValueError(f"pages hold 'compute' or 'e4m3', not {kind!r}")
+        if kind == "e4m3":
+            lacking = [what for what, there in (("biases and norms over whole projections", self.prologue), ("keys kept behind a window", self.keep_first),
+                                                ("a cap on the scores", self.score_cap is not None), ("slopes", self.slope_list is not None)) if there]
+            if lacking:
+                raise ValueError(f"attention over an 8-bit cache has no {' and no '.join(lacking)}")
+            if self.head_dim % 16 or not 16 <= self.head_dim <= 256:
+                raise ValueError(f"attention over an 8-bit cache takes head sizes in steps of 16 up to 256, not {self.head_dim}")
+        self.pages_hold = kind
+
     def cache_need(self):
+        if self.pages_hold == "e4m3":
+            return CacheNeed.keys_and_values_e4m3(self.num_kv_heads, self.head_dim, self.window, self.chunk)
         return CacheNeed.keys_and_values(self.num_kv_heads, self.head_dim, self.window, self.chunk, self.keep_first)
 
     def set_param(self, local, tensor):
@@ -299,6 +317,11 @@ class Attention(Mixer):
         kw = self.k_norm_weight if (self.qk_norm_eps is not None and self.own_kv) else qw
         table = self.position.rotary_table() if self.position is not None else None
         eps = self.qk_norm_eps or 0.0
+        if self.pages_hold == "e4m3":
+            o = self._attend_e4m3(qkv, qw, kw, eps, table, step, cache, store)
+            if self.head_gate:
+                ops.head_gate(o, packed[:, self.gate_at:self.gate_at + Hq], Hq, D)
+            return self._project(o, packed)
         if (store and step.num_decodes == step.num_tokens and (self.position is None or table is not None)
                 and plain_scores and ops.decode_step_fuses(qkv.dtype, D, cache.page_size)):
             # only single tokens: norm, rotary, cache write and attention in one launch
@@ -341,6 +364,36 @@ class Attention(Mixer):
         if gated:
             ops.head_gate(o, packed[:, self.gate_at:self.gate_at + Hq], Hq, D)
         return self._project(o, packed)
+
+    def _attend_e4m3(self, qkv, qw, kw, eps, table, step, cache, store):
+        """Norm, position, the write of this step's keys and values and attention, over pages of 8 bits."""
+        Hq, Hkv, D = self.num_heads, self.num_kv_heads, self.head_dim
+        grp = step.groups[cache.group]
+        pages = ops.PagesE4M3(cache.k, cache.v, cache.tensors["k_scales"], cache.tensors["v_scales"])
+        bound = max(step.max_decode_context, step.max_prefill_context)
+        q = qkv[:, : self.q_size]
+        if self.position is not None and table is None:
+            # a position encoding that has no table: norm in place, its own apply, then the write as it is
+            if self.values_are_keys:
+                raise NotImplementedError("values that are the keys need a position encoding with a table, or none")
+            nk = Hkv if self.own_kv else 0
+            ops.qk_norm_rope_store(qkv[:, : self.q_size + nk * D], qw, kw, eps, None, step.positions, None, None, None, Hq, nk, D,
+                                   cache.page_size, store=False)
+            T = qkv.shape[0]
+            self.position.apply(q.view(T, Hq, D), qkv[:, self.q_size: self.q_size + nk * D].view(T, nk, D), step.positions)
+            if store:
+                ops.qk_norm_rope_store_e4m3(qkv[:, self.q_size:], None, None, 0.0, None, step.positions, grp.slot_mapping, pages, 0, Hkv, D,
+                                            cache.page_size)
+        elif store:
+            q = ops.qk_norm_rope_store_e4m3(qkv, qw, kw, eps, table, step.positions, grp.slot_mapping, pages, Hq, Hkv, D, cache.page_size,
+                                            position_bound=bound, values_are_keys=self.values_are_keys)
+        else:
+            ops.qk_norm_rope_store(q, qw, kw, eps, table, step.positions, None, None, None, Hq, 0, D, cache.page_size, store=False,
+                                   position_bound=bound)
+        return ops.paged_attention_e4m3(q, pages, cache.page_size, grp.block_tables, step.context_lens, step.seq_of_token, step.positions,
+                                        step.prefill_cu, step.num_decodes, step.max_decode_context, self.scale, self.window, Hq, Hkv, D,
+                                        max_prefill_context=step.max_prefill_context, even_contexts=step.decode_contexts_even,
+                                        chunk=self.chunk, sinks=self.sinks)
 
     def _project(self, o, packed):
         """The element gate, the output product and its bias."""

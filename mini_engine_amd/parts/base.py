@@ -43,18 +43,22 @@ class PageTensor:
     like, with PAGE where the page's tokens are counted: keys stored token by token under their head
     are (heads, PAGE, head size); values transposed inside a page are (heads, head size, PAGE); one
     latent vector per token is (PAGE, width). The pool allocates [pages, *shape] with PAGE replaced by
-    the engine's page size. `dtype`: "compute" (the engine's), "float32", "bfloat16" or "int32"."""
+    the engine's page size. `dtype`: "compute" (the engine's), "float32", "bfloat16", "int32", "e4m3" or "uint8".
+    `tokens`: so many of a page's tokens share an entry (a block's scale); pages are multiples of it."""
 
     name: str
     shape: tuple
     dtype: str = "compute"
+    tokens: int = 1
 
     def __post_init__(self):
         if sum(1 for d in self.shape if d == PAGE) != 1:
             raise ValueError(f"page tensor {self.name!r}: exactly one axis of {self.shape} must be PAGE")
 
     def sized(self, page_size: int) -> tuple:
-        return tuple(page_size if d == PAGE else int(d) for d in self.shape)
+        if page_size % self.tokens:
+            raise ValueError(f"page tensor {self.name!r}: pages of {page_size} tokens are no multiple of {self.tokens}")
+        return tuple(page_size // self.tokens if d == PAGE else int(d) for d in self.shape)
 
 
 @dataclass(frozen=True)
@@ -82,6 +86,13 @@ class CacheNeed:
         size, page] (V transposed inside a page: the P.V operand of the matrix cores is then one load)."""
         return cls((PageTensor("k", (num_kv_heads, PAGE, head_dim)), PageTensor("v", (num_kv_heads, head_dim, PAGE))),
                    window, chunk, keep_first=int(keep_first or 0))
+
+    @classmethod
+    def keys_and_values_e4m3(cls, num_kv_heads: int, head_dim: int, window: int | None = None, chunk: int | None = None) -> "CacheNeed":
+        """The same in 8 bits: e4m3 numbers, and for every 16 tokens and head a byte that names their power of two."""
+        scale = (num_kv_heads, PAGE)
+        return cls((PageTensor("k", (num_kv_heads, PAGE, head_dim), "e4m3"), PageTensor("v", (num_kv_heads, head_dim, PAGE), "e4m3"),
+                    PageTensor("k_scales", scale, "uint8", 16), PageTensor("v_scales", scale, "uint8", 16)), window, chunk)
 
     def own_rule(self) -> tuple:
         """("window", n), ("chunk", c) or ("all", 0)."""

@@ -209,3 +209,46 @@ def attention_bound(o, spread):
 def place_bound(exact, powers):
     """A stored number against what it rounds: half a step, 2^-4 of it or 2^-10 of its power below the normal numbers; 2e-6 of float32 work."""
     return (2.0 ** -4 + 2e-6) * exact.abs() + 2.0 ** -10 * torch.exp2(powers.double()) + 1e-30
+
+
+# ------------------------------------------------------------------ the engine's bookkeeping without a GPU
+
+def _write_back(plain: PlainPages, pages) -> None:
+    pages.k.view(torch.uint8).copy_(plain.k.to(torch.float8_e4m3fn).view(torch.uint8))
+    pages.v.view(torch.uint8).copy_(plain.v.to(torch.float8_e4m3fn).view(torch.uint8))
+    pages.k_scales.copy_((plain.kp + BIAS).to(torch.uint8))
+    pages.v_scales.copy_((plain.vp + BIAS).to(torch.uint8))
+
+
+class PlainOps:
+    """The two operators on tensors anywhere, through the plain forms above; beside `kernel_twins.PlainBackend` for the rest."""
+
+    calls = 0
+
+    @staticmethod
+    def qk_norm_rope_store_e4m3(rows, q_weight, k_weight, eps, table, positions, slots, pages, Hq, Hkv, D, page, position_bound=0, values_are_keys=False):
+        PlainOps.calls += 1
+        assert table is None or position_bound <= table.shape[0]
+        assert pages.check("append", Hkv, D, page) == pages.k.shape[0]
+        on = lambda t: None if t is None else t.cpu()  # noqa: E731
+        heads = rows.cpu().double().view(rows.shape[0], -1, D)
+        q = normed_rotated(heads[:, :Hq], on(q_weight), eps, on(table), positions.cpu())
+        k = normed_rotated(heads[:, Hq:Hq + Hkv], on(k_weight), eps, on(table), positions.cpu())
+        plain = PlainPages.of(pages)
+        plain.place(k, heads[:, Hq:Hq + Hkv] if values_are_keys else heads[:, Hq + Hkv:], slots.tolist())
+        _write_back(plain, pages)
+        return q.reshape(rows.shape[0], Hq * D).to(rows)
+
+    @staticmethod
+    def paged_attention_e4m3(q, pages, page, block_tables, context_lens, seq_of_token, positions, prefill_cu, num_decodes, max_decode_context, scale,
+                             window, Hq, Hkv, D, max_prefill_context=0, even_contexts=False, chunk=None, sinks=None):
+        contexts = context_lens.tolist()
+        cu = list(range(num_decodes)) + [num_decodes + c for c in (prefill_cu.tolist() if prefill_cu is not None else [0])]
+        new = [b - a for a, b in zip(cu, cu[1:])]
+        assert max(contexts[:num_decodes], default=0) <= max_decode_context and max(contexts[num_decodes:], default=0) <= max_prefill_context
+        step = Step.__new__(Step)
+        step.new, step.page, step.contexts = new, page, torch.tensor(contexts)
+        step.table_rows = [[int(p) if 0 <= p < pages.k.shape[0] else -1 for p in row] for row in block_tables.tolist()]
+        o, _ = attend(q.cpu().double().view(q.shape[0], Hq, D), PlainPages.of(pages).numbers(), step, scale, Hq, Hkv, window, chunk,
+                      None if sinks is None else sinks.cpu())
+        return o.reshape(q.shape).to(q)

@@ -240,6 +240,14 @@ def test_attention_mixed_step(Hq, Hkv, D, page):
     _check_attention(MIX, Hq, Hkv, D, page, seed=D, gap=8)
 
 
+@pytest.mark.parametrize("Hq,Hkv,D", [(16, 8, 128), (6, 2, 32), (5, 1, 48), (8, 8, 80), (8, 2, 64), (40, 2, 128), (3, 3, 256)])
+def test_attention_of_portions(Hq, Hkv, D):
+    """Tiles that end inside a wave, blocks before, on and behind the diagonal, more than 32 blocks (whose pages are looked up anew)."""
+    lengths = [(2, 0), (65, 0), (7, 130), (129, 16), (300, 1500), (257, 31)]
+    _check_attention(lengths, Hq, Hkv, D, 16, seed=D)
+    _check_attention(lengths, Hq, Hkv, D, 64, seed=D, window=200, sinks=torch.randn(Hq, generator=_gen(1)))
+
+
 @pytest.mark.parametrize("options", [dict(window=1), dict(window=16), dict(window=63), dict(window=100), dict(chunk=8), dict(chunk=50), dict(window=40, sinks=True),
                                      dict(sinks=True), dict(chunk=64, sinks=True)])
 @pytest.mark.parametrize("Hq,Hkv,D", [(4, 2, 64), (8, 8, 32)])
@@ -259,6 +267,20 @@ def test_attention_long(lengths, window):
 def test_attention_uneven_scores():
     """Loud queries: a few keys have all of the softmax, and the maximum rises again and again."""
     got, o, _ = _check_attention(MIX + [(200, 900)], 4, 2, 64, 16, seed=3, loud=20.0)
+
+
+@pytest.mark.parametrize("D", [32, 128, 256])
+def test_attention_nan_in_a_value(D):
+    """A value that is NaN makes NaN of its channel in the rows that see it and of nothing else, on the diagonal, in front of it, under a window
+    and where the range is cut into partitions."""
+    for new, before, at, window in ((90, 0, 50, None), (70, 700, 720, None), (70, 700, 100, None), (60, 100, 130, 20), (40, 3000, 2999, None)):
+        def pages(step, gen):
+            p = mild_pages(step.pages, 2, D, 16, gen)
+            p.v.view(torch.uint8)[step.table_rows[0][at // 16], 1, 7, at % 16] = 0x7F
+            return p
+        got, o, step = _check_attention([(new, before)], 4, 2, D, 16, seed=5, pages=pages, window=window)
+        seen = sum(1 for i in range(before, before + new) if at <= i and not (window and at <= i - window))
+        assert int(torch.isnan(got).sum()) == seen * 2 and torch.isnan(got[:, 2:, 7]).sum() == seen * 2
 
 
 def test_attention_nan_where_nobody_looks():
