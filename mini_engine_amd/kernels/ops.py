@@ -381,26 +381,35 @@ class PagesE4M3:
         """Raises unless the tensors are such pages; returns how many there are."""
         _check(page >= self.BLOCK and page & (page - 1) == 0, f"{what}: a page has a power of two of tokens, 16 or more, not {page}")
         _check(D % 16 == 0 and 16 <= D <= 256, f"{what}: the head size must be a multiple of 16 up to 256, not {D}")
-        k, v, n = self.k, self.v, self.k.shape[0] if self.k.dim() else 0
-        if not (n >= 1 and k.shape == (n, Hkv, page, D) and v.shape == (n, Hkv, D, page) and k.dtype == v.dtype == torch.float8_e4m3fn
+        k, v = self.k, self.v
+        shape = k.shape
+        n = shape[0] if shape else 0
+        if not (n >= 1 and shape == (n, Hkv, page, D) and v.shape == (n, Hkv, D, page) and k.dtype == v.dtype == torch.float8_e4m3fn
                 and k.is_contiguous() and v.is_contiguous()):
             raise KernelError(f"{what}: pages must be contiguous e4m3 numbers, K [pages, Hkv, page, D] and V [pages, Hkv, D, page]")
+        blocks = (n, Hkv, page // self.BLOCK)
         for t in (self.k_scales, self.v_scales):
-            _check(t.dtype == torch.uint8 and t.shape == (n, Hkv, page // self.BLOCK) and t.is_contiguous(),
-                   f"{what}: the blocks' powers must be contiguous uint8 [pages, Hkv, page / 16]")
+            if not (t.dtype == torch.uint8 and t.shape == blocks and t.is_contiguous()):
+                raise KernelError(f"{what}: the blocks' powers must be contiguous uint8 [pages, Hkv, page / 16]")
         return n
 
     def tensors(self) -> tuple:
         return self.k, self.v, self.k_scales, self.v_scales
 
 
-def _check_device(what: str, *tensors) -> None:
-    """All on the GPU that launches go to: the kernels run on the current device's current stream."""
+def _check_device(what: str, *tensors) -> int:
+    """All on the GPU that launches go to: the kernels run on the current device's current stream, whose handle this returns."""
+    here = tensors[0].get_device()
+    if here >= 0 and here == torch._C._cuda_getDevice():
+        for t in tensors:
+            if t is not None and t.get_device() != here:
+                break
+        else:
+            return _raw_stream(here) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
     _require_gpu()
     here = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and not (t.is_cuda and t.device.index == here):
-            raise KernelError(f"{what}: every tensor must be on the current GPU (cuda:{here}), got one on {t.device}")
+    where = next(t.device for t in tensors if t is not None and t.get_device() != here)
+    raise KernelError(f"{what}: every tensor must be on the current GPU (cuda:{here}), got one on {where}")
 
 
 class HipBackend:
@@ -697,27 +706,32 @@ class HipBackend:
         other in another order are taken as calls one after the other; a block whose rows stand apart in one call holds either of them.
         slots below 0 or beyond the pages are skipped. (reference models/qwen3.py:34-36, layers/rotary_embedding.py:20-25,
         csrc/kv_cache.cu:10-31, whose cache has the activations' type.)"""
-        what = "qk_norm_rope_store_e4m3"
-        _check(rows.dtype == torch.bfloat16, f"{what}: rows must be bfloat16, got {rows.dtype}")
+        what = "qk_norm_rope_store_e4m3"          # (messages are formed where they are needed)
+        if rows.dtype != torch.bfloat16:
+            raise KernelError(f"{what}: rows must be bfloat16, got {rows.dtype}")
         T = rows.shape[0]
         width = (Hq + (1 if values_are_keys else 2) * Hkv) * D
         if not (rows.dim() == 2 and rows.stride(1) == 1 and rows.shape[1] == width and (T <= 1 or rows.stride(0) >= width)):
             raise KernelError(f"{what}: rows must be [T, {width}] with unit inner stride, got {tuple(rows.shape)}")
-        _check(Hq >= 0 and Hkv >= 1, f"{what}: bad head counts")
+        if not (Hq >= 0 and Hkv >= 1):
+            raise KernelError(f"{what}: bad head counts")
         n = pages.check(what, Hkv, D, page)
         for w in (q_weight, k_weight):
-            _check(w is None or (w.dtype == torch.float32 and w.shape == (D,) and w.is_contiguous()), f"{what}: norm weights must be float32 [D]")
-        _check((q_weight is None) == (k_weight is None), f"{what}: give both norm weights or neither")
+            if not (w is None or (w.dtype == torch.float32 and w.shape == (D,) and w.is_contiguous())):
+                raise KernelError(f"{what}: norm weights must be float32 [D]")
+        if (q_weight is None) != (k_weight is None):
+            raise KernelError(f"{what}: give both norm weights or neither")
         if table is not None:
-            _check(table.dtype == torch.float32 and table.is_contiguous() and table.dim() == 3 and table.shape[1:] == (D // 2, 2),
-                   f"{what}: rotary table must be float32 [P, D/2, 2]")
-        _check(_is_i32(positions, T) and _is_i32(slots, T), f"{what}: positions and slots must be int32 [T]")
-        _check_device(what, rows, q_weight, k_weight, table, positions, slots, *pages.tensors())
+            if not (table.dtype == torch.float32 and table.is_contiguous() and table.dim() == 3 and table.shape[1:] == (D // 2, 2)):
+                raise KernelError(f"{what}: rotary table must be float32 [P, D/2, 2]")
+        if not (_is_i32(positions, T) and _is_i32(slots, T)):
+            raise KernelError(f"{what}: positions and slots must be int32 [T]")
+        stream = _check_device(what, rows, q_weight, k_weight, table, positions, slots, *pages.tensors())
         q = torch.empty((T, Hq * D), dtype=rows.dtype, device=rows.device)
         core().call("me_append_e4m3", rows.data_ptr(), max(rows.stride(0), width), q.data_ptr(), _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(table),
                     0 if table is None else table.shape[0], int(position_bound), positions.data_ptr(), slots.data_ptr(), pages.k.data_ptr(),
                     pages.v.data_ptr(), pages.k_scales.data_ptr(), pages.v_scales.data_ptr(), n, T, Hq, Hkv, D, page,
-                    int(bool(values_are_keys)), _stream())
+                    int(bool(values_are_keys)), stream)
         return q
 
     def paged_attention_e4m3(self, q, pages: PagesE4M3, page: int, block_tables, context_lens, seq_of_token, positions, prefill_cu,
@@ -731,20 +745,27 @@ class HipBackend:
         a power of two from 16 on. Returns [T, Hq*D]. (reference layers/attention.py:63-76, over a cache of the activations' type.)"""
         what = "paged_attention_e4m3"
         T, B = q.shape[0], context_lens.numel()
-        _check(q.dtype == torch.bfloat16, f"{what}: queries must be bfloat16, got {q.dtype}")
-        _check(q.dim() == 2 and q.shape[1] == Hq * D and q.stride(1) == 1 and (T <= 1 or q.stride(0) >= Hq * D),
-               f"{what}: q must be [T, Hq*D], unit inner stride")
+        if q.dtype != torch.bfloat16:
+            raise KernelError(f"{what}: queries must be bfloat16, got {q.dtype}")
+        if not (q.dim() == 2 and q.shape[1] == Hq * D and q.stride(1) == 1 and (T <= 1 or q.stride(0) >= Hq * D)):
+            raise KernelError(f"{what}: q must be [T, Hq*D], unit inner stride")
         n = pages.check(what, Hkv, D, page)
-        _check(block_tables.dim() == 2 and block_tables.dtype == torch.int32 and block_tables.stride(1) == 1 and block_tables.shape[0] >= B
-               and block_tables.shape[1] >= 1, f"{what}: block tables must be int32 [B, MB]")
-        _check(_is_i32(context_lens) and _is_i32(seq_of_token, T) and _is_i32(positions, T), f"{what}: metadata must be int32")
-        _check(0 <= num_decodes <= B and num_decodes <= T, f"{what}: bad decode count")
-        _check(not (window and chunk), f"{what}: a window and a block mask exclude each other")
-        _check((window or 0) >= 0 and (chunk or 0) >= 0, f"{what}: a window or a block must not be negative")
-        _check(sinks is None or (sinks.dtype == torch.float32 and sinks.shape == (Hq,) and sinks.is_contiguous()), f"{what}: sinks must be float32 [Hq]")
-        _check(T == num_decodes or (B > num_decodes and prefill_cu is not None and _is_i32(prefill_cu, B - num_decodes + 1)),
-               f"{what}: prefill_cu must be int32 [B-Dn+1]")
-        _check_device(what, q, block_tables, context_lens, prefill_cu, sinks, *pages.tensors())
+        if not (block_tables.dim() == 2 and block_tables.dtype == torch.int32 and block_tables.stride(1) == 1 and block_tables.shape[0] >= B
+                and block_tables.shape[1] >= 1):
+            raise KernelError(f"{what}: block tables must be int32 [B, MB]")
+        if not (_is_i32(context_lens) and _is_i32(seq_of_token, T) and _is_i32(positions, T)):
+            raise KernelError(f"{what}: metadata must be int32")
+        if not (0 <= num_decodes <= B and num_decodes <= T):
+            raise KernelError(f"{what}: bad decode count")
+        if window and chunk:
+            raise KernelError(f"{what}: a window and a block mask exclude each other")
+        if not ((window or 0) >= 0 and (chunk or 0) >= 0):
+            raise KernelError(f"{what}: a window or a block must not be negative")
+        if not (sinks is None or (sinks.dtype == torch.float32 and sinks.shape == (Hq,) and sinks.is_contiguous())):
+            raise KernelError(f"{what}: sinks must be float32 [Hq]")
+        if not (T == num_decodes or (B > num_decodes and prefill_cu is not None and _is_i32(prefill_cu, B - num_decodes + 1))):
+            raise KernelError(f"{what}: prefill_cu must be int32 [B-Dn+1]")
+        stream = _check_device(what, q, block_tables, context_lens, prefill_cu, sinks, *pages.tensors())
         out = torch.empty((T, Hq * D), dtype=q.dtype, device=q.device)
         if T == 0:
             return out
@@ -758,7 +779,7 @@ class HipBackend:
             scratch = torch.empty(num_decodes * Hq * parts * (D + 2), dtype=torch.float32, device=q.device) if parts > 1 else None
             lib.call("me_attn8_decode", q.data_ptr(), rows, out.data_ptr(), Hq * D, *pools, block_tables.data_ptr(), *tables,
                      context_lens.data_ptr(), num_decodes, Hq, Hkv, page, float(scale), int(window or 0), int(chunk or 0), part, parts,
-                     _ptr(scratch), _ptr(sinks), _stream())
+                     _ptr(scratch), _ptr(sinks), stream)
         if T > num_decodes:
             Tp = T - num_decodes
             part, parts = prompt_partitions_e4m3(Tp, B - num_decodes, Hq, Hkv, D, max_prefill_context or block_tables.shape[1] * page, span)
@@ -766,7 +787,7 @@ class HipBackend:
             lib.call("me_attn8_prompt", q.data_ptr() + num_decodes * rows * 2, rows, out.data_ptr() + num_decodes * Hq * D * 2, Hq * D, *pools,
                      block_tables.data_ptr() + num_decodes * tables[0] * 4, *tables, context_lens.data_ptr() + num_decodes * 4,
                      prefill_cu.data_ptr(), Tp, B - num_decodes, Hq, Hkv, page, float(scale), int(window or 0), int(chunk or 0), part, parts,
-                     _ptr(scratch), _ptr(sinks), _stream())
+                     _ptr(scratch), _ptr(sinks), stream)
         return out
 
     # -- matrix products -----------------------------------------------------------------
