@@ -100,6 +100,8 @@ __device__ __forceinline__ float power_of(uint32_t byte) { return __uint_as_floa
 struct Pages {
   int k, v;            // table entries as loaded
 };
+// Keys and values of single tokens are read once: marked as not to be kept by the caches, which the memory system answers with a higher rate.
+__device__ __forceinline__ u32x4v stream16(const uint8_t* p) { return __builtin_nontemporal_load(reinterpret_cast<const u32x4v*>(p)); }
 struct Block {
   u32x4v k[4][KL], v[DT];
   uint32_t kcode, vcode;
@@ -114,24 +116,26 @@ __device__ __forceinline__ Pages find_pages(const Attn8Args& a, const int32_t* _
   p.v = table[group_in(vk, lo, L) ? vk >> a.page_shift : 0];
   return p;
 }
-__device__ __forceinline__ void load_block(const Attn8Args& a, const Pages& p, int kvh, int t0, int lo, int L, int n, int g, Block& b) {
-  const int mask = (1 << a.page_shift) - 1;
-  const int kk = t0 + 16 * (n >> 2), vk = t0 + 16 * g;
-  const bool kok = group_in(kk, lo, L) && (unsigned)p.k < (unsigned)a.num_pages;
-  b.there = group_in(vk, lo, L) && (unsigned)p.v < (unsigned)a.num_pages;
-  const int64_t kh = (int64_t)(kok ? p.k : 0) * a.Hkv + kvh, vh = (int64_t)(b.there ? p.v : 0) * a.Hkv + kvh;
-  const int koff = kk & mask, voff = vk & mask;
-  const uint8_t* kp = a.k + ((kh << a.page_shift) + koff + (n & 3)) * HD + 16 * g;
+__device__ __forceinline__ void load_keys(const Attn8Args& a, const Pages& p, int kvh, int t0, int lo, int L, int n, int g, Block& b) {
+  const int kk = t0 + 16 * (n >> 2), off = kk & ((1 << a.page_shift) - 1);
+  const bool ok = group_in(kk, lo, L) && (unsigned)p.k < (unsigned)a.num_pages;
+  const int64_t at = (int64_t)(ok ? p.k : 0) * a.Hkv + kvh;
+  const uint8_t* from = a.k + ((at << a.page_shift) + off + (n & 3)) * HD + 16 * g;
 #pragma unroll
   for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
     for (int j = 0; j < KL; ++j)
-      b.k[tt][j] = *reinterpret_cast<const u32x4v*>(kp + tt * 4 * HD + ((HD % 64 == 0 || 64 * j + 16 * g < HD) ? 64 * j : -16 * g));
-  const uint8_t* vp = a.v + ((vh * HD + n) << a.page_shift) + voff;
+      b.k[tt][j] = stream16(from + tt * 4 * HD + ((HD % 64 == 0 || 64 * j + 16 * g < HD) ? 64 * j : -16 * g));
+  b.kcode = a.k_powers[(at << (a.page_shift - 4)) + (off >> 4)];
+}
+__device__ __forceinline__ void load_values(const Attn8Args& a, const Pages& p, int kvh, int t0, int lo, int L, int n, int g, Block& b) {
+  const int vk = t0 + 16 * g, off = vk & ((1 << a.page_shift) - 1);
+  b.there = group_in(vk, lo, L) && (unsigned)p.v < (unsigned)a.num_pages;
+  const int64_t at = (int64_t)(b.there ? p.v : 0) * a.Hkv + kvh;
+  const uint8_t* from = a.v + ((at * HD + n) << a.page_shift) + off;
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) b.v[dt] = *reinterpret_cast<const u32x4v*>(vp + ((int64_t)(16 * dt) << a.page_shift));
-  b.kcode = a.k_powers[(kh << (a.page_shift - 4)) + (koff >> 4)];
-  b.vcode = a.v_powers[(vh << (a.page_shift - 4)) + (voff >> 4)];
+  for (int dt = 0; dt < DT; ++dt) b.v[dt] = stream16(from + ((int64_t)(16 * dt) << a.page_shift));
+  b.vcode = a.v_powers[(at << (a.page_shift - 4)) + (off >> 4)];
 }
 
 // The queries of one column, in the order of the channels that load_block gives a lane.
@@ -210,10 +214,12 @@ __device__ __forceinline__ void softmax_tiles(const f32x4* st, float sc, int fir
   c.l[ct] += sum;
 }
 
-// One block out of registers, for a wave's single column tile. FULL: every column sees every key of it, and all of them lie in pages.
-// (Otherwise all columns see the same keys: what none of them sees is zeroed, and a NaN among the others is everybody's.)
-template <bool FULL>
-__device__ __forceinline__ void attend(const Attn8Args& a, Block& b, int t0, int lo, int L, int g, const bf16x8 (&q)[2 * KL], Columns<1>& c) {
+// One block out of registers, for a wave's single column tile; more_keys and more_values ask for the next one's, each as soon as this one's
+// have been used, into the same registers. FULL: every column sees every key of it, and all of them lie in pages. (Otherwise all columns
+// see the same keys: what none of them sees is zeroed, and a NaN among the others is everybody's.)
+template <bool FULL, typename K, typename V>
+__device__ __forceinline__ void attend(const Attn8Args& a, Block& b, int t0, int lo, int L, int g, const bf16x8 (&q)[2 * KL], Columns<1>& c, K more_keys,
+                                       V more_values) {
   const float kpow = power_of(b.kcode), vpow = power_of(b.vcode);
   f32x4 st[4];
 #pragma unroll
@@ -229,6 +235,7 @@ __device__ __forceinline__ void attend(const Attn8Args& a, Block& b, int t0, int
     }
     st[tt] = s;
   }
+  more_keys();
   bf16x8 pb[2];
   uint32_t seen;
   softmax_tiles<1, FULL, 4>(st, a.scale * LOG2E, t0 + 16 * g, b.there, 0, c, seen, pb);
@@ -238,6 +245,7 @@ __device__ __forceinline__ void attend(const Attn8Args& a, Block& b, int t0, int
 #pragma unroll
     for (int h = 0; h < 2; ++h)
       c.acc[0][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(b.v[dt][2 * h], b.v[dt][2 * h + 1], vpow), pb[h], c.acc[0][dt], 0, 0, 0);
+  more_values();
 }
 
 // A softmax's denominator with its head's sink; a column that saw no key stays at zero.
@@ -248,23 +256,32 @@ __device__ __forceinline__ float inverse(float d) { return d == 0.f ? 0.f : 1.f 
 
 // =====================================================================================
 // Single tokens. Grid (key heads x column tiles, requests, partitions): the 4 waves of a workgroup take the 64-key blocks of a
-// partition in turn and are merged through LDS.
+// partition in turn and are merged through LDS. A request has as many partitions as its keys need; the workgroups of others leave at once
+// and write nothing. The last partitions come first: only long requests have them. A block's keys are asked for when its predecessor's
+// have been multiplied, its values when the predecessor's have been: into the same registers (two blocks in registers of their own left
+// no room for the sums, 8 requests of 32,768 keys 110 us for 98).
 // =====================================================================================
-__global__ void __launch_bounds__(256) attn8_decode_kernel(Attn8Args a) {
+__device__ __forceinline__ int parts_of(const Attn8Args& a, int L) {      // of a request with L keys: 1 at least
+  const int base = L > 0 ? first_seen(a, L - 1) & ~(BK - 1) : 0;
+  return a.num_parts == 1 ? 1 : min(a.num_parts, max(1, (L - base + a.part_keys - 1) / a.part_keys));
+}
+
+__global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attn8_decode_kernel(Attn8Args a) {
   extern __shared__ float lds[];      // [4 waves][columns][HD + 2]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
-  const int b = blockIdx.y, part = blockIdx.z;
+  const int b = blockIdx.y, part = a.num_parts - 1 - blockIdx.z;
+  const int L = context_of(a, b), pos = L - 1;
+  if (part >= parts_of(a, L)) return;
   const int col_tiles = (a.G + 15) / 16;
   const int kvh = blockIdx.x / col_tiles, ctile = blockIdx.x - kvh * col_tiles;
-  const int L = context_of(a, b), pos = L - 1;
   const int lo = L > 0 ? first_seen(a, pos) : 0;
   const int base = lo & ~(BK - 1);
   const int p_lo = base + part * a.part_keys, p_hi = part + 1 < a.num_parts ? min(p_lo + a.part_keys, L) : L;      // (the last one takes what the host did not know of)
   const int ncols = min(16, a.G - ctile * 16);
   const bool valid = n < ncols;
   const int head = kvh * a.G + ctile * 16 + (valid ? n : 0);
-  const int32_t* table = a.tables + (int64_t)b * a.table_stride;
+  const int32_t* __restrict__ table = a.tables + (int64_t)b * a.table_stride;
   Columns<1> c;
   c.m[0] = NONE; c.l[0] = 0.f;
   c.lo[0] = lo; c.hi[0] = valid ? pos : -1;
@@ -272,19 +289,24 @@ __global__ void __launch_bounds__(256) attn8_decode_kernel(Attn8Args a) {
   for (int dt = 0; dt < DT; ++dt) c.acc[0][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   int t0 = p_lo + BK * wave;
   if (t0 < p_hi) {
+    constexpr int STEP = 4 * BK;
+    Block blk;
+    Pages pages = find_pages(a, table, t0, lo, L, n, g);
     bf16x8 q[2 * KL];
     load_q(a.q + b * a.q_stride + (int64_t)head * HD, valid, g, q);
-
-    Block blk;
-    load_block(a, find_pages(a, table, t0, lo, L, n, g), kvh, t0, lo, L, n, g, blk);
+    load_keys(a, pages, kvh, t0, lo, L, n, g, blk);
+    load_values(a, pages, kvh, t0, lo, L, n, g, blk);
     while (true) {
+      // the next block's table entries, looked up while this one's keys are on their way
+      const bool more = t0 + STEP < p_hi;
+      if (more) pages = find_pages(a, table, t0 + STEP, lo, L, n, g);
+      auto more_keys = [&]() { if (more) load_keys(a, pages, kvh, t0 + STEP, lo, L, n, g, blk); };
+      auto more_values = [&]() { if (more) load_values(a, pages, kvh, t0 + STEP, lo, L, n, g, blk); };
       // a block whose pages are all there and whose keys the token sees: whole-wave test
-      const bool full = t0 >= lo && t0 + BK <= p_hi && __all(blk.there);
-      if (full) attend<true>(a, blk, t0, lo, L, g, q, c);
-      else attend<false>(a, blk, t0, lo, L, g, q, c);
-      t0 += 4 * BK;
-      if (t0 >= p_hi) break;
-      load_block(a, find_pages(a, table, t0, lo, L, n, g), kvh, t0, lo, L, n, g, blk);
+      if (t0 >= lo && t0 + BK <= p_hi && __all(blk.there)) attend<true>(a, blk, t0, lo, L, g, q, c, more_keys, more_values);
+      else attend<false>(a, blk, t0, lo, L, g, q, c, more_keys, more_values);
+      if (!more) break;
+      t0 += STEP;
     }
   }
   const float l = sum_of_column(c.l[0]);
@@ -750,34 +772,50 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
       }
 }
 
-// Joins the partitions of a (row, head): out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p. A wave to a (row, head); partitions
-// without a key (l = 0) are not read.
+// Joins the partitions of a (row, head): out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p. A wave to a (row, head): a lane weighs a
+// partition, then all of them sum the channels, eight partitions asked for at a time. DECODE: row t is request t, which may have fewer.
+template <bool DECODE>
 __global__ void __launch_bounds__(256) attn8_join_kernel(Attn8Args a, int64_t rows) {
   const int lane = threadIdx.x & 63;
   const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (at >= rows * a.Hq) return;
   const int64_t t = at / a.Hq;
   const int head = (int)(at - t * a.Hq);
-  const float* ml = a.part_ml + 2 * at * a.num_parts;
+  const int parts = DECODE ? parts_of(a, context_of(a, (int)t)) : a.num_parts;
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + at * a.num_parts;
   const float* po = a.part_o + at * a.num_parts * HD;
+  constexpr int CH = (HD + 63) / 64;
   float M = NONE;
-  for (int p = lane; p < a.num_parts; p += 64) M = fmaxf(M, ml[2 * p]);
+  for (int p = lane; p < parts; p += 64) M = fmaxf(M, ml[p].x);
   M = wave_max(M);
-  float sum = 0.f, o[(HD + 63) / 64];
+  float sum = 0.f, o[CH];
 #pragma unroll
-  for (int j = 0; j < (HD + 63) / 64; ++j) o[j] = 0.f;
-  for (int p = 0; p < a.num_parts; ++p) {
-    const float l = ml[2 * p + 1];
-    if (l == 0.f) continue;
-    const float f = exp2f(ml[2 * p] - M);
-    sum += f * l;
+  for (int j = 0; j < CH; ++j) o[j] = 0.f;
+  for (int p0 = 0; p0 < parts; p0 += 64) {
+    const float2 mine = p0 + lane < parts ? ml[p0 + lane] : make_float2(NONE, 0.f);
+    const float f = mine.y == 0.f ? 0.f : exp2f(mine.x - M);      // (no key: nothing, whatever the maxima)
+    sum += wave_sum(f * mine.y);
+    const int upto = min(64, parts - p0);
+    for (int i = 0; i < upto; i += 8) {
+      float v[8][CH];
 #pragma unroll
-    for (int j = 0; j < (HD + 63) / 64; ++j)
-      if (lane + 64 * j < HD) o[j] += f * po[(int64_t)p * HD + lane + 64 * j];
+      for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int j = 0; j < CH; ++j) {
+          const int d = lane + 64 * j;
+          v[e][j] = po[(int64_t)(p0 + min(i + e, upto - 1)) * HD + (HD % 64 == 0 || d < HD ? d : 0)];
+        }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float fe = i + e < upto ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), i + e)) : 0.f;
+#pragma unroll
+        for (int j = 0; j < CH; ++j) o[j] = i + e < upto ? fmaf(fe, v[e][j], o[j]) : o[j];
+      }
+    }
   }
   const float inv = inverse(with_sink(a, head, M, sum));
 #pragma unroll
-  for (int j = 0; j < (HD + 63) / 64; ++j)
+  for (int j = 0; j < CH; ++j)
     if (lane + 64 * j < HD) a.out[t * a.out_stride + (int64_t)head * HD + lane + 64 * j] = static_cast<bf16_t>(o[j] * inv);
 }
 
@@ -814,9 +852,10 @@ static int fill(Attn8Args& a, const void* q, int64_t q_stride, void* out, int64_
   return 0;
 }
 
+template <bool DECODE>
 static int join(const Attn8Args& a, int64_t rows, hipStream_t stream) {
   if (a.num_parts == 1) return 0;
-  attn8_join_kernel<<<(unsigned)((rows * a.Hq + 3) / 4), 256, 0, stream>>>(a, rows);
+  attn8_join_kernel<DECODE><<<(unsigned)((rows * a.Hq + 3) / 4), 256, 0, stream>>>(a, rows);
   ME_LAUNCH_CHECK();
   return 0;
 }
@@ -838,7 +877,7 @@ extern "C" int me_attn8_decode(const void* q, int64_t q_stride, void* out, int64
   dim3 grid(a.Hkv * ((a.G + 15) / 16), num_seqs, num_parts);
   attn8_decode_kernel<<<grid, 256, lds, stream>>>(a);
   ME_LAUNCH_CHECK();
-  return join(a, num_seqs, stream);
+  return join<true>(a, num_seqs, stream);
 }
 
 extern "C" int me_attn8_prompt(const void* q, int64_t q_stride, void* out, int64_t out_stride, const void* k, const void* v,
@@ -858,5 +897,5 @@ extern "C" int me_attn8_prompt(const void* q, int64_t q_stride, void* out, int64
   }
   attn8_prompt_kernel<<<dim3((unsigned)(tiles * Hkv), num_parts), 256, LDS_BYTES, stream>>>(a, (int)tiles);
   ME_LAUNCH_CHECK();
-  return join(a, rows, stream);
+  return join<false>(a, rows, stream);
 }
