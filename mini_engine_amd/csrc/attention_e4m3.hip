@@ -365,12 +365,15 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attn8_decode_kernel(At
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int COLS = 128;                    // columns of a tile
 constexpr int PB = 32;                       // keys of a block
-constexpr int KS = HD / 16;                  // products of a tile of scores
+constexpr int CB = (HD + 31) / 32;           // products of a tile of scores: 64 numbers of a column's query against as many of the keys
+constexpr int KC = (CB + 1) / 2;             // operands of keys
 constexpr int DC = (HD + 31) / 32;           // channel tiles of the values
-constexpr int KBUF = 2 * KS * PB * 16, VBUF = 4 * DC * 32 * 16;
+constexpr int VBUF = 4 * DC * 32 * 16;
 constexpr int PIECES = (HD + 127) / 128;     // 16-byte pieces of keys (and of values) of a block that a lane brings
 constexpr int RAW = 4 * 1024 * PIECES;       // bytes of a block's keys (and of its values) as they come
-constexpr int AT_RAW = 0, AT_K = 8 * RAW, AT_V = AT_K + 2 * KBUF, AT_FLAGS = AT_V + 3 * VBUF, LDS_BYTES = AT_FLAGS + 16;      // (keys begin at multiples of 256)
+constexpr int KRAW = RAW + 256;              // the second 16 keys 128 bytes further on
+constexpr int AT_K = 0, AT_RAW = 8 * KRAW, AT_V = AT_RAW + 4 * RAW, AT_FLAGS = AT_V + 3 * VBUF, LDS_BYTES = AT_FLAGS + 16;
+typedef int i32x8 __attribute__((ext_vector_type(8)));
 static_assert(LDS_BYTES <= 160 * 1024 && (HD > 128 || 2 * LDS_BYTES <= 160 * 1024), "one workgroup to a compute unit, two up to head size 128");
 
 // 64 x 16 bytes from base + voff (bytes, per lane) to LDS at lds_addr + 16 * lane. The write to m0 needs one wait state before an
@@ -466,16 +469,49 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
   const int64_t row = q0 + tok;
   float m = NONE, l = 0.f;
   const int lo = valid ? first_seen(a, max(start + tok, 0)) : 0, hi = valid ? start + tok : -1;      // the keys that the column sees
-  bf16x8 q[KS];
+  // The column's query as two e4m3 numbers each under one power, x = (high + low / 16) 2^p with |high| < 256: what rounding to high leaves of a
+  // bfloat16 has 4 bits, so the two are exact for numbers down to 2^-14 of the largest and off by 2^-22 of the largest below.
+  i32x8 q[CB];
+  uint32_t q_powers;                          // of high, of low; in the third byte, of high in the lower lanes and of low in the upper ones
   {
-    const bf16_t* from = a.q + row * a.q_stride + (int64_t)head * HD + 8 * h;
+    const bf16_t* from = a.q + row * a.q_stride + (int64_t)head * HD;
+    uint4 raw[KC][4];                         // channels 64 j + 32 h ..: a lane's 32; of an odd last 32 a lane has 16
+    uint32_t top = 0;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      bf16x8 x = *reinterpret_cast<const bf16x8*>(from + 16 * ks);
+    for (int j = 0; j < KC; ++j)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = valid ? x[e] : static_cast<bf16_t>(0.f);
-      q[ks] = x;
-    }
+      for (int e = 0; e < 4; ++e) {
+        if (2 * j + 1 == CB && e >= 2) break;
+        const int c = 64 * j + (2 * j + 1 < CB ? 32 : 16) * h + 8 * e;
+        uint4 x = *reinterpret_cast<const uint4*>(from + (c < HD ? c : 0));
+        if (!valid || c >= HD) x = make_uint4(0, 0, 0, 0);
+        raw[j][e] = x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { const uint32_t w = (&x.x)[i]; top = max(top, max(w & 0x7fffu, (w >> 16) & 0x7fffu)); }
+      }
+    const auto both = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+    const int power = min(max((int)(max(both[0], both[1]) >> 7) - 7, 4), 247);      // the largest number between 128 and 256 of it
+    const float down = __uint_as_float((uint32_t)(254 - power) << 23);
+    q_powers = (uint32_t)power | (uint32_t)(power - 4) << 8 | (uint32_t)(power - (h ? 4 : 0)) << 16;
+#pragma unroll
+    for (int j = 0; j < KC; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {           // four channels at a time
+        if (2 * j + 1 == CB && e >= 4) break;
+        const uint32_t w[2] = {(&raw[j][e >> 1].x)[2 * (e & 1)], (&raw[j][e >> 1].x)[2 * (e & 1) + 1]};
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16) * down;
+        int high = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+        high = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], high, true);
+        float r[4];
+        r[0] = (x[0] - __builtin_amdgcn_cvt_f32_fp8(high, 0)) * 16.f; r[1] = (x[1] - __builtin_amdgcn_cvt_f32_fp8(high, 1)) * 16.f;
+        r[2] = (x[2] - __builtin_amdgcn_cvt_f32_fp8(high, 2)) * 16.f; r[3] = (x[3] - __builtin_amdgcn_cvt_f32_fp8(high, 3)) * 16.f;
+        int low = __builtin_amdgcn_cvt_pk_fp8_f32(r[0], r[1], 0, false);
+        low = __builtin_amdgcn_cvt_pk_fp8_f32(r[2], r[3], low, true);
+        if (2 * j + 1 < CB) { q[2 * j][e] = high; q[(2 * j + 1) % CB][e] = low; }
+        else { q[2 * j][e] = high; q[2 * j][(4 + e) & 7] = low; }
+      }
   }
   f32x16 acc[DC];
 #pragma unroll
@@ -500,56 +536,41 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
     auto ask_codes = [&](int t0, int ids) -> uint32_t {
       const int off = (t0 + 16 * lane) & page_mask;
       const int64_t at = (((int64_t)max(ids, 0) * a.Hkv + kvh) << (a.page_shift - 4)) + (off >> 4);
-      return code_of(a.k_powers[at]) << 23 | code_of(a.v_powers[at]) << 15;      // the power itself, and another 8 bits further right
+      return code_of(a.k_powers[at]) | code_of(a.v_powers[at]) << 23;      // as the products take it, and the power itself
     };
     uint32_t codes = ask_codes(seg_lo, pages), more_codes = 0;
     const uint32_t lds0 = (uint32_t)(uintptr_t)lds_bytes;
-    const uint32_t mine = 16 * lane + 1024 * PIECES * wave;     // where this lane's pieces lie in a block's bytes
-    // Block k's bytes to slot k % 4 (beyond the last block: page 0's, which is always there). A lane's keys: row lane % 8 of the wave's
+    const uint32_t mine = 16 * lane + 1024 * PIECES * wave;     // where this lane's values lie in a block's bytes
+    // Block k's keys to slot k % 8, its values to slot k % 4 (beyond the last block: page 0's, which is always there). A lane's keys: row lane % 8 of the wave's
     // 8, 16 channels; its values: a channel.
     const uint32_t page_bytes = (uint32_t)(a.Hkv * HD) << a.page_shift;
     const uint8_t* k_head = a.k + (((int64_t)kvh << a.page_shift) + 8 * part) * HD;
     const uint8_t* v_head = a.v + (((int64_t)kvh * HD + part * (HD / 2)) << a.page_shift);
     const uint32_t k_lane = (lane & 7) * HD + (lane >> 3) * 16, v_lane = (uint32_t)lane << a.page_shift;
-    const uint32_t my_slot = lds0 + AT_RAW + 1024 * PIECES * wave;
+    const uint32_t my_keys = lds0 + AT_K + 1024 * PIECES * wave + 128 * group, my_values = lds0 + AT_RAW + 1024 * PIECES * wave;
     auto offset_of = [&](int k) { return (seg_lo + PB * k + 16 * group) & page_mask; };
     auto page_of = [&](int k) { return (uint64_t)(uint32_t)max(__builtin_amdgcn_readlane(pages, (2 * k + group) & 63), 0) * page_bytes; };
     auto bring_keys = [&](int k, uint64_t page) {
 #pragma unroll
       for (int i = 0; i < PIECES; ++i)
-        if (HD % 128 == 0 || lane + 64 * i < HD / 2) bring16(k_head + page + offset_of(k) * HD + 128 * i, k_lane, my_slot + (k & 3) * (2 * RAW) + 1024 * i);
+        if (HD % 128 == 0 || lane + 64 * i < HD / 2) bring16(k_head + page + offset_of(k) * HD + 128 * i, k_lane, my_keys + (k & 7) * KRAW + 1024 * i);
     };
     auto bring_values = [&](int k, uint64_t page) {
 #pragma unroll
       for (int i = 0; i < PIECES; ++i)
         if (HD % 128 == 0 || lane + 64 * i < HD / 2)
-          bring16(v_head + page + offset_of(k) + ((int64_t)(64 * i) << a.page_shift), v_lane, my_slot + (k & 3) * (2 * RAW) + RAW + 1024 * i);
+          bring16(v_head + page + offset_of(k) + ((int64_t)(64 * i) << a.page_shift), v_lane, my_values + (k & 3) * RAW + 1024 * i);
     };
-    u32x4v raw_k[PIECES], raw_v[PIECES];
-    auto read_raw_keys = [&](int k) {
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i) raw_k[i] = *reinterpret_cast<const u32x4v*>(lds_bytes + AT_RAW + (k & 3) * (2 * RAW) + mine + 1024 * i);
-    };
+    u32x4v raw_v[PIECES];
     auto read_raw_values = [&](int k) {
 #pragma unroll
-      for (int i = 0; i < PIECES; ++i) raw_v[i] = *reinterpret_cast<const u32x4v*>(lds_bytes + AT_RAW + (k & 3) * (2 * RAW) + RAW + mine + 1024 * i);
-    };
-    // Half j of a block's keys as bfloat16. Of the wave's 8 keys 16 group + 8 part + r: row 16 group + 8 (r / 4) + 4 part + r % 4; channels
-    // 16 c + 8 j ..: piece 2 c + j.
-    auto store_keys = [&](int j, uint32_t code, char* kbuf) {
-      const float power = __uint_as_float(code & 0x7f800000u);
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i) {
-        const int r = lane & 7, c = (lane >> 3) + 8 * i;
-        char* to = kbuf + (2 * c * PB + ((16 * group + 8 * (r >> 2) + 4 * part + (r & 3)) ^ (4 * ((c >> 1) & 1)))) * 16;
-        if (HD % 128 == 0 || 16 * c < HD) *reinterpret_cast<bf16x8*>(to + 16 * PB * j) = operand(raw_k[i][2 * j], raw_k[i][2 * j + 1], power);
-      }
+      for (int i = 0; i < PIECES; ++i) raw_v[i] = *reinterpret_cast<const u32x4v*>(lds_bytes + AT_RAW + (k & 3) * RAW + mine + 1024 * i);
     };
     // Half j of block k's values. Keys in front of tile_lo, or from L on, or in no page become zeros; a NaN among the others is reported.
     // WHOLE: every column of the tile sees all of the block, and it lies in pages.
     auto store_values = [&](auto whole_tag, int j, int k, uint32_t code, uint32_t there, char* vbuf) {
       constexpr bool WHOLE = decltype(whole_tag)::value;
-      const float power = __uint_as_float((code << 8) & 0x7f800000u);
+      const float power = __uint_as_float(code & 0x7f800000u);
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
         const int p = lane + 64 * i;
@@ -577,12 +598,34 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
 
     const float sc = a.scale * LOG2E;
     const uint32_t rd_v = AT_V + (32 * DC * h + n) * 16;
-    // pieces 2 ks + h: the rows' fours change places where ks / 2 is odd
-    const uint32_t rd_k[2] = {(uint32_t)(AT_K + (h * PB + n) * 16), (uint32_t)(AT_K + (h * PB + (n ^ 4)) * 16)};
-    bf16x8 ka[KS];
-    auto read_keys = [&](uint32_t buf) {
+    // A lane's row stands for key 16 (n / 16) + 8 (n / 4 % 2) + 4 (n / 8 % 2) + n % 4; its channels are 64 j + 32 h .. + 31, of an odd last 32
+    // the 16 h-th 16, twice (zeros beyond the head's)
+    const uint32_t rd_k = AT_K + 1024 * PIECES * (2 * (n >> 4) + ((n >> 2) & 1)) + 128 * (n >> 4) + 16 * ((n & 3) + 4 * ((n >> 3) & 1));
+    union Keys { i32x8 all; u32x4v half[2]; };
+    Keys ka[KC];
+    auto read_keys = [&](int k) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) ka[ks] = *reinterpret_cast<const bf16x8*>(lds_bytes + buf + rd_k[(ks >> 1) & 1] + 2 * ks * PB * 16);
+      for (int j = 0; j < KC; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const bool odd = 2 * j + 1 == CB;
+          if (odd && e) { ka[j].half[1] = ka[j].half[0]; break; }
+          const int piece = 4 * j + (odd ? h : 2 * h + e), last = 4 * j + (odd ? 1 : 2 + e);      // (of the upper lanes)
+          const u32x4v w = *reinterpret_cast<const u32x4v*>(lds_bytes + (k & 7) * KRAW + rd_k + 1024 * (j / 2) + 128 * (piece & 7));
+          ka[j].half[e] = 16 * last < HD || 16 * piece < HD ? w : u32x4v{0, 0, 0, 0};
+        }
+    };
+    // product i of a tile of scores: high and low of 64 channels in turn, or both of 32 (a lane's power is for 32 of the 64 numbers: those in
+    // the first four registers of both halves of the lanes, or those in the last four)
+    uint32_t k_powers = 0;
+    auto score = [&](int i, const f32x16& c) {
+      if (i / 2 * 2 + 1 >= CB) return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(ka[i / 2].all, q[i], c, 0, 0, 0, (int)k_powers, 2, (int)q_powers);
+      if (i % 2 == 0) return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(ka[i / 2].all, q[i], c, 0, 0, 0, (int)k_powers, 0, (int)q_powers);
+      return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(ka[i / 2].all, q[i], c, 0, 0, 0, (int)k_powers, 1, (int)q_powers);
+    };
+    auto powers_of_block = [&](int k) {       // of the lane's key
+      const uint32_t first = __builtin_amdgcn_readlane(codes, (2 * k) & 63), second = __builtin_amdgcn_readlane(codes, (2 * k + 1) & 63);
+      return n < 16 ? first : second;
     };
     const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     f32x16 st;                                // the scores of the block whose softmax comes next
@@ -598,26 +641,18 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
     brought<3 * PIECES>();
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      read_raw_keys(k); read_raw_values(k);
+      read_raw_values(k);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        store_keys(j, code_of_block(k), lds_bytes + AT_K + k * KBUF);
-        store_values(std::false_type{}, j, k, code_of_block(k), there_of(k), lds_bytes + AT_V + k * VBUF);
-      }
+      for (int j = 0; j < 2; ++j) store_values(std::false_type{}, j, k, code_of_block(k), there_of(k), lds_bytes + AT_V + k * VBUF);
     }
-    read_raw_keys(2);
     step_barrier();
     bring_keys(4, page_of(4)); bring_keys(5, page_of(5)); bring_values(4, page_of(4));
     read_keys(0);
-    __builtin_amdgcn_sched_barrier(0);
+    k_powers = powers_of_block(0);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[ks], q[ks], ks ? st : zero, 0, 0, 0);
-    read_keys(KBUF);
-    step_barrier();
-#pragma unroll
-    for (int j = 0; j < 2; ++j) store_keys(j, code_of_block(2), lds_bytes + AT_K);
-    step_barrier();
-    uint32_t code_v = code_of_block(2);       // of the block whose values are turned into bfloat16 next
+    for (int i = 0; i < CB; ++i) st = score(i, i ? st : zero);
+    read_keys(1);
+    k_powers = powers_of_block(1);
     uint64_t page_v = page_of(5);             // of the block whose values are asked for next
 
     uint32_t cur = 0, nxt = VBUF, to = 2 * VBUF;        // the values of blocks k, k + 1, k + 2
@@ -628,9 +663,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
       const int t0 = seg_lo + PB * k;
       const uint32_t there = hist & 3;
       brought<4 * PIECES>();                  // keys of block k + 3, values of k + 2; the two steps' after them are still on their way
-      read_raw_keys(k + 3);
       read_raw_values(k + 2);
-      const uint32_t code_k = code_of_block(k + 3);
+      const uint32_t code_v = code_of_block(k + 2), next_powers = powers_of_block(k + 2);
       bf16x8 va[2 * DC];                      // keys 16 j + 8 h .. of channel tile dt: DC j + dt
       auto read_values = [&](int from, int upto) {
 #pragma unroll
@@ -675,7 +709,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
         if (i == 8) { __builtin_amdgcn_sched_barrier(0); read_values(0, DC); }
         if (i == 12) { __builtin_amdgcn_sched_barrier(0); read_values(DC, 2 * DC); }
 #pragma unroll
-        for (int ks = i * KS / 16; ks < (i + 1) * KS / 16; ++ks) sn = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[ks], q[ks], ks ? sn : zero, 0, 0, 0);
+        for (int j = 0; j < CB; ++j)
+          if (i == 16 * j / CB) { sn = score(j, j ? sn : zero); asm volatile("" : "+v"(sn)); __builtin_amdgcn_sched_barrier(0); }
         float p = __builtin_amdgcn_exp2f(fmaf(st[i], sc, -m));
         if constexpr (!FULL) p = sees(i) ? p : 0.f;      // while a column has seen no key, its reference point is NONE too
         sum = i ? sum + p : p;
@@ -684,25 +719,19 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
       }
       __builtin_amdgcn_sched_barrier(0);
       l += sum;
-      char *kbuf = lds_bytes + AT_K + ((k + 1) & 1) * KBUF, *vbuf = lds_bytes + AT_V + to;
+      char* vbuf = lds_bytes + AT_V + to;
 #pragma unroll
       for (int i = 0; i < 2 * DC; ++i) {
-        if (i == DC) { __builtin_amdgcn_sched_barrier(0); read_keys((k & 1) * KBUF); }      // block k + 2's, where half of the values' have been used
+        if (i == DC) { __builtin_amdgcn_sched_barrier(0); read_keys(k + 2); }      // where half of the values' have been used
         acc[i % DC] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[i], pb[i / DC], acc[i % DC], 0, 0, 0);
         if constexpr (STEADY) {
 #pragma unroll
-          for (int j = i * 2 / DC; j < (i + 1) * 2 / DC; ++j) {
-            if (j < 2) store_keys(j, code_k, kbuf);
-            else store_values(std::true_type{}, j - 2, k + 2, code_v, 3, vbuf);
-          }
+          for (int j = i / DC; j < (i + 1) / DC; ++j) store_values(std::true_type{}, j, k + 2, code_v, 3, vbuf);
         }
       }
       if constexpr (!STEADY) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          store_keys(j, code_k, kbuf);
-          store_values(std::false_type{}, j, k + 2, code_v, (hist >> 4) & 3, vbuf);
-        }
+        for (int j = 0; j < 2; ++j) store_values(std::false_type{}, j, k + 2, code_v, (hist >> 4) & 3, vbuf);
       }
       // (what is held for 32 blocks is stored whether it has changed or not: a store in each branch would put it into scratch memory)
       const int next = k + 6, t_next = seg_lo + PB * next;
@@ -710,13 +739,13 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
       uint32_t now_codes = codes, later_codes = more_codes;
       if (__builtin_expect((next & 31) == 31, 0)) { asm volatile("" ::: "memory"); later = ask_pages(t_next + PB); }
       if (__builtin_expect((next & 31) == 0, 0)) { asm volatile("" ::: "memory"); now = settle_pages(t_next, later); later_codes = ask_codes(t_next, now); held = __ballot(now >= 0); }
-      if (__builtin_expect((next & 31) == 2, 0)) now_codes = later_codes;          // the next step turns block k + 4's keys into bfloat16, the first of its 32
+      if (__builtin_expect((next & 31) == 3, 0)) now_codes = later_codes;          // the next step looks up block k + 3's, the first of its 32
       pages = now; more_pages = later; codes = now_codes; more_codes = later_codes;
       hist = hist >> 2 | there_of(next) << 10;
       const uint64_t page_k = page_of(next);
       bring_keys(next, page_k);
       bring_values(next - 1, page_v);
-      page_v = page_k; code_v = code_k;
+      page_v = page_k; k_powers = next_powers;
       st = sn;
       const uint32_t free = cur;
       cur = nxt; nxt = to; to = free;
