@@ -34,6 +34,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 // log2 units by which a column's maximum must rise before its sums are rescaled: probabilities then reach 2^8 instead of 1, which
 // neither float32 sums nor bfloat16's relative rounding minds, and blocks after a tile's first hardly ever rescale.
 constexpr float RESCALE_STEP = 8.f;
+constexpr float MOST_WEIGHT = 4096.f;          // ... and, of prompts, the sum of a lane's weights of a block up to which it stays
 
 struct Attn8Args {
   const bf16_t* q;
@@ -526,40 +527,57 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
     const int group = wave >> 1, part = wave & 1;             // this wave brings half of a block's 16 keys `group`: 8 keys, HD / 2 channels of values
     const int page_mask = (1 << a.page_shift) - 1;
     if (threadIdx.x == 0) *nan_flag = 0;
-    // The pages of 32 blocks are held by the wave's lanes, one for every 16 keys, and a block's are read from there.
+    // What 32 blocks need is held by the wave's lanes, one for every 16 keys, and a block's read from there: where its bytes lie (page 0 where
+    // no page is), behind the wave's own pieces of keys and of values, and the powers (asked for when the pages are known).
+    const uint32_t page_bytes = (uint32_t)(a.Hkv * HD) << a.page_shift;
     auto ask_pages = [&](int t0) { const int key = t0 + 16 * lane; return table[group_in(key, tile_lo, L) ? key >> a.page_shift : 0]; };
     auto settle_pages = [&](int t0, int raw) { return group_in(t0 + 16 * lane, tile_lo, L) && (unsigned)raw < (unsigned)a.num_pages ? raw : -1; };
-    int pages = settle_pages(seg_lo, ask_pages(seg_lo)), more_pages = 0;
-    uint64_t held = __ballot(pages >= 0);
-    auto there_of = [&](int k) { return (uint32_t)(held >> ((2 * k) & 63)) & 3u; };      // bit i: the block's 16 keys i lie in a page
-    // The powers of the same blocks, keys' and values' in one number, a lane for every 16 keys (asked for when the pages are known).
+    struct Where { uint32_t k_lo, k_hi, v_lo, v_hi; };
+    auto find = [&](int t0, int ids) {
+      const uint64_t page = (uint64_t)(uint32_t)max(ids, 0) * page_bytes;
+      const int off = (t0 + 16 * lane) & page_mask;
+      const uint64_t k = page + off * HD, v = page + off;
+      return Where{(uint32_t)k, (uint32_t)(k >> 32), (uint32_t)v, (uint32_t)(v >> 32)};
+    };
     auto ask_codes = [&](int t0, int ids) -> uint32_t {
       const int off = (t0 + 16 * lane) & page_mask;
       const int64_t at = (((int64_t)max(ids, 0) * a.Hkv + kvh) << (a.page_shift - 4)) + (off >> 4);
       return code_of(a.k_powers[at]) | code_of(a.v_powers[at]) << 23;      // as the products take it, and the power itself
     };
-    uint32_t codes = ask_codes(seg_lo, pages), more_codes = 0;
+    int more_pages = settle_pages(seg_lo, ask_pages(seg_lo));
+    Where at = find(seg_lo, more_pages);
+    uint32_t codes = ask_codes(seg_lo, more_pages), more_codes = 0;
+    // bits 2 k and 2 k + 1: block k's groups lie in pages; of the last 32 blocks looked up and of the 32 before
+    uint64_t held = __ballot(more_pages >= 0), held_before = 0;
+    // the first block from tile_from on that does not wholly lie in pages, as far as is known
+    const int first_whole = max(tile_from - seg_lo + PB - 1, 0) / PB;
+    auto clear_upto = [&](int k0) {
+      const int skip = first_whole - k0;
+      const uint64_t missing = skip >= 32 ? 0 : ~held & (~0ull << (2 * max(skip, 0)));
+      return k0 + (missing ? __builtin_ctzll(missing) / 2 : 32);
+    };
+    int clear = clear_upto(0);
     const uint32_t lds0 = (uint32_t)(uintptr_t)lds_bytes;
     const uint32_t mine = 16 * lane + 1024 * PIECES * wave;     // where this lane's values lie in a block's bytes
-    // Block k's keys to slot k % 8, its values to slot k % 4 (beyond the last block: page 0's, which is always there). A lane's keys: row lane % 8 of the wave's
-    // 8, 16 channels; its values: a channel.
-    const uint32_t page_bytes = (uint32_t)(a.Hkv * HD) << a.page_shift;
+    // Block k's keys to slot k % 8, its values to slot k % 4 (beyond the last block: page 0's, which is always there). A lane's keys: row
+    // lane % 8 of the wave's 8, 16 channels; its values: a channel.
     const uint8_t* k_head = a.k + (((int64_t)kvh << a.page_shift) + 8 * part) * HD;
     const uint8_t* v_head = a.v + (((int64_t)kvh * HD + part * (HD / 2)) << a.page_shift);
     const uint32_t k_lane = (lane & 7) * HD + (lane >> 3) * 16, v_lane = (uint32_t)lane << a.page_shift;
     const uint32_t my_keys = lds0 + AT_K + 1024 * PIECES * wave + 128 * group, my_values = lds0 + AT_RAW + 1024 * PIECES * wave;
-    auto offset_of = [&](int k) { return (seg_lo + PB * k + 16 * group) & page_mask; };
-    auto page_of = [&](int k) { return (uint64_t)(uint32_t)max(__builtin_amdgcn_readlane(pages, (2 * k + group) & 63), 0) * page_bytes; };
-    auto bring_keys = [&](int k, uint64_t page) {
+    auto held_at = [&](uint32_t x, int k) { return (uint32_t)__builtin_amdgcn_readlane(x, (2 * k + group) & 63); };
+    auto keys_of = [&](int k) { return (uint64_t)held_at(at.k_hi, k) << 32 | held_at(at.k_lo, k); };
+    auto values_of = [&](int k) { return (uint64_t)held_at(at.v_hi, k) << 32 | held_at(at.v_lo, k); };
+    auto bring_keys = [&](int k, uint64_t from) {
 #pragma unroll
       for (int i = 0; i < PIECES; ++i)
-        if (HD % 128 == 0 || lane + 64 * i < HD / 2) bring16(k_head + page + offset_of(k) * HD + 128 * i, k_lane, my_keys + (k & 7) * KRAW + 1024 * i);
+        if (HD % 128 == 0 || lane + 64 * i < HD / 2) bring16(k_head + from + 128 * i, k_lane, my_keys + (k & 7) * KRAW + 1024 * i);
     };
-    auto bring_values = [&](int k, uint64_t page) {
+    auto bring_values = [&](int k, uint64_t from) {
 #pragma unroll
       for (int i = 0; i < PIECES; ++i)
         if (HD % 128 == 0 || lane + 64 * i < HD / 2)
-          bring16(v_head + page + offset_of(k) + ((int64_t)(64 * i) << a.page_shift), v_lane, my_values + (k & 3) * RAW + 1024 * i);
+          bring16(v_head + from + ((int64_t)(64 * i) << a.page_shift), v_lane, my_values + (k & 3) * RAW + 1024 * i);
     };
     u32x4v raw_v[PIECES];
     auto read_raw_values = [&](int k) {
@@ -594,7 +612,6 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
         }
       }
     };
-    auto code_of_block = [&](int k) { return (uint32_t)__builtin_amdgcn_readlane(codes, (2 * k + group) & 63); };
 
     const float sc = a.scale * LOG2E;
     const uint32_t rd_v = AT_V + (32 * DC * h + n) * 16;
@@ -623,48 +640,43 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
       if (i % 2 == 0) return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(ka[i / 2].all, q[i], c, 0, 0, 0, (int)k_powers, 0, (int)q_powers);
       return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(ka[i / 2].all, q[i], c, 0, 0, 0, (int)k_powers, 1, (int)q_powers);
     };
-    auto powers_of_block = [&](int k) {       // of the lane's key
-      const uint32_t first = __builtin_amdgcn_readlane(codes, (2 * k) & 63), second = __builtin_amdgcn_readlane(codes, (2 * k + 1) & 63);
-      return n < 16 ? first : second;
-    };
+    const int power_lane = 4 * (n >> 4);
+    auto powers_of_block = [&](int k) { return (uint32_t)__builtin_amdgcn_ds_bpermute(power_lane + ((8 * k) & 255), (int)codes); };      // of the lane's key
     const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    f32x16 st;                                // the scores of the block whose softmax comes next
+    f32x16 scores, scores_next;               // of the block whose softmax comes next, of the one after
 
     // What the first step finds: block 0's scores, block 1's keys in registers and block 2's in LDS, the values of 0 and 1 in LDS, and on their
     // way, in this order, the keys and values of (3, 2), (4, 3), (5, 4).
-    uint32_t hist = 0;                        // two bits for every block from the current one on: its groups in pages
-#pragma unroll
-    for (int k = 0; k < 6; ++k) hist |= there_of(k) << (2 * k);
-    bring_keys(0, page_of(0)); bring_keys(1, page_of(1)); bring_values(0, page_of(0)); bring_values(1, page_of(1)); bring_keys(2, page_of(2));
-    bring_keys(3, page_of(3)); bring_values(2, page_of(2)); bring_values(3, page_of(3));
+    bring_keys(0, keys_of(0)); bring_keys(1, keys_of(1)); bring_values(0, values_of(0)); bring_values(1, values_of(1)); bring_keys(2, keys_of(2));
+    bring_keys(3, keys_of(3)); bring_values(2, values_of(2)); bring_values(3, values_of(3));
     step_barrier();                           // (the flag)
     brought<3 * PIECES>();
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       read_raw_values(k);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) store_values(std::false_type{}, j, k, code_of_block(k), there_of(k), lds_bytes + AT_V + k * VBUF);
+      for (int j = 0; j < 2; ++j) store_values(std::false_type{}, j, k, held_at(codes, k), (uint32_t)(held >> (2 * k)), lds_bytes + AT_V + k * VBUF);
     }
     step_barrier();
-    bring_keys(4, page_of(4)); bring_keys(5, page_of(5)); bring_values(4, page_of(4));
+    bring_keys(4, keys_of(4)); bring_keys(5, keys_of(5)); bring_values(4, values_of(4));
     read_keys(0);
     k_powers = powers_of_block(0);
 #pragma unroll
-    for (int i = 0; i < CB; ++i) st = score(i, i ? st : zero);
+    for (int i = 0; i < CB; ++i) scores = score(i, i ? scores : zero);
     read_keys(1);
     k_powers = powers_of_block(1);
-    uint64_t page_v = page_of(5);             // of the block whose values are asked for next
+    uint64_t values_at = values_of(5);        // of the block whose values are asked for next
 
     uint32_t cur = 0, nxt = VBUF, to = 2 * VBUF;        // the values of blocks k, k + 1, k + 2
+    auto there_of = [&](int b, int k) { return (uint32_t)(((b >> 5) == ((k + 5) >> 5) ? held : held_before) >> ((2 * b) & 63)) & 3u; };      // block b's groups, in step k
     // STEADY: every column of the wave sees every key of block k, every one of the tile those of block k + 2, and both lie in pages; such a
     // step has no branch but for a maximum that rises and for what is held for the next 32 blocks.
-    auto step = [&](auto steady_tag, int k) {
+    auto step = [&](auto steady_tag, int k, const f32x16& st, f32x16& sn) {
       constexpr bool STEADY = decltype(steady_tag)::value, FULL = STEADY;
       const int t0 = seg_lo + PB * k;
-      const uint32_t there = hist & 3;
       brought<4 * PIECES>();                  // keys of block k + 3, values of k + 2; the two steps' after them are still on their way
       read_raw_values(k + 2);
-      const uint32_t code_v = code_of_block(k + 2), next_powers = powers_of_block(k + 2);
+      const uint32_t code_v = held_at(codes, k + 2), next_powers = powers_of_block(k + 2);
       bf16x8 va[2 * DC];                      // keys 16 j + 8 h .. of channel tile dt: DC j + dt
       auto read_values = [&](int from, int upto) {
 #pragma unroll
@@ -676,33 +688,22 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
       if constexpr (!FULL) {
         const int from = max(lo - t0, 0), upto = min(hi - t0, 31);
         const uint32_t range = upto >= from && from < 32 ? (uint32_t)((2ull << upto) - (1ull << from)) : 0u;
+        const uint32_t there = there_of(k, k);
         seen = (range & ((there & 1 ? 0xffffu : 0u) | (there & 2 ? 0xffff0000u : 0u))) >> (8 * h);
       }
       auto sees = [&](int i) { return (seen >> (i < 8 ? i : i + 8)) & 1; };
-      float top = NONE;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        if constexpr (!FULL) st[i] = sees(i) ? st[i] : NONE;
-        top = fmaxf(top, st[i]);
-      }
-      if (__builtin_expect(__any((top > 0.5f * NONE) & (top * sc > m + RESCALE_STEP)), 0)) {
-        const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-        const float t = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
-        const float next = t > 0.5f * NONE ? t * sc : NONE;
-        // (a branch of the lanes, not of the wave: the sums are scaled in the registers that they are in)
-        if (next > m + RESCALE_STEP) {
-          const float f = __builtin_amdgcn_exp2f(m - next);
-          l *= f;
-#pragma unroll
-          for (int dt = 0; dt < DC; ++dt)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[dt][i] *= f;
-          m = next;
-        }
-      }
-      f32x16 sn;
       bf16x8 pb[2];
-      float sum = 0.f, even = 0.f;
+      auto weigh = [&](int i) {               // (while a column has seen no key, its reference point is NONE: infinite)
+        const float p = __builtin_amdgcn_exp2f(fmaf(st[i], sc, -m));
+        return FULL || sees(i) ? p : 0.f;
+      };
+      auto sum_up = [&]() {                   // of the weights as they are rounded
+        float s[2] = {0.f, 0.f};
+        const bf16x2 ones = {static_cast<bf16_t>(1.f), static_cast<bf16_t>(1.f)};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i & 1] = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{pb[i >> 2][2 * (i & 3)], pb[i >> 2][2 * (i & 3) + 1]}, ones, s[i & 1], false);
+        return s[0] + s[1];
+      };
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         // the values' operands take the registers of the keys' that have been used
@@ -711,11 +712,29 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
 #pragma unroll
         for (int j = 0; j < CB; ++j)
           if (i == 16 * j / CB) { sn = score(j, j ? sn : zero); asm volatile("" : "+v"(sn)); __builtin_amdgcn_sched_barrier(0); }
-        float p = __builtin_amdgcn_exp2f(fmaf(st[i], sc, -m));
-        if constexpr (!FULL) p = sees(i) ? p : 0.f;      // while a column has seen no key, its reference point is NONE too
-        sum = i ? sum + p : p;
-        if (i & 1) { pb[i >> 3][(i & 7) - 1] = static_cast<bf16_t>(even); pb[i >> 3][i & 7] = static_cast<bf16_t>(p); }
-        else even = p;
+        pb[i >> 3][i & 7] = static_cast<bf16_t>(weigh(i));
+      }
+      float sum = sum_up();
+      // The reference point is raised only when a weight got large, and the block's weights are taken again.
+      if (__builtin_expect(__any(sum > MOST_WEIGHT), 0)) {
+        float top = NONE;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, FULL || sees(i) ? st[i] * sc : NONE);
+        const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+        const float next = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+        // (a branch of the lanes, not of the wave: the sums are scaled in the registers that they are in)
+        if (next > m) {
+          const float f = __builtin_amdgcn_exp2f(m - next);
+          l *= f;
+#pragma unroll
+          for (int dt = 0; dt < DC; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[dt][i] *= f;
+          m = next;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) pb[i >> 3][i & 7] = static_cast<bf16_t>(weigh(i));
+        sum = sum_up();
       }
       __builtin_amdgcn_sched_barrier(0);
       l += sum;
@@ -731,34 +750,41 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
       }
       if constexpr (!STEADY) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) store_values(std::false_type{}, j, k + 2, code_v, (hist >> 4) & 3, vbuf);
+        for (int j = 0; j < 2; ++j) store_values(std::false_type{}, j, k + 2, code_v, there_of(k + 2, k), vbuf);
       }
       // (what is held for 32 blocks is stored whether it has changed or not: a store in each branch would put it into scratch memory)
-      const int next = k + 6, t_next = seg_lo + PB * next;
-      int now = pages, later = more_pages;
+      const int next = k + 6;
+      Where now = at;
+      int later = more_pages;
       uint32_t now_codes = codes, later_codes = more_codes;
-      if (__builtin_expect((next & 31) == 31, 0)) { asm volatile("" ::: "memory"); later = ask_pages(t_next + PB); }
-      if (__builtin_expect((next & 31) == 0, 0)) { asm volatile("" ::: "memory"); now = settle_pages(t_next, later); later_codes = ask_codes(t_next, now); held = __ballot(now >= 0); }
-      if (__builtin_expect((next & 31) == 3, 0)) now_codes = later_codes;          // the next step looks up block k + 3's, the first of its 32
-      pages = now; more_pages = later; codes = now_codes; more_codes = later_codes;
-      hist = hist >> 2 | there_of(next) << 10;
-      const uint64_t page_k = page_of(next);
-      bring_keys(next, page_k);
-      bring_values(next - 1, page_v);
-      page_v = page_k; k_powers = next_powers;
-      st = sn;
+      if (__builtin_expect(((next + 1) & 31) < 5, 0)) {
+        asm volatile("" ::: "memory");
+        const int t_next = seg_lo + PB * next;
+        if ((next & 31) == 31) later = ask_pages(t_next + PB);
+        if ((next & 31) == 0) {
+          later = settle_pages(t_next, later);
+          now = find(t_next, later); later_codes = ask_codes(t_next, later);
+          held_before = held; held = __ballot(later >= 0);
+          if (clear == next) clear = clear_upto(next);
+        }
+        if ((next & 31) == 3) now_codes = later_codes;      // the next step looks up block k + 3's, the first of its 32
+      }
+      at = now; more_pages = later; codes = now_codes; more_codes = later_codes;
+      bring_keys(next, keys_of(next));
+      bring_values(next - 1, values_at);
+      values_at = values_of(next); k_powers = next_powers;
       const uint32_t free = cur;
       cur = nxt; nxt = to; to = free;
       step_barrier();
     };
     // Blocks are walked in ascending order: in front of the window's first whole block, those that the wave sees whole (steady as long as every
     // group has its page), the rest. Loops of their own: where the ways through a step meet, the sums would change their registers.
-    const int first_steady = max(all_lo - seg_lo + PB - 1, 0) / PB, first_whole = max(tile_from - seg_lo + PB - 1, 0) / PB;
-    const int end_steady = all_hi >= seg_lo && tile_upto >= seg_lo ? min(min((all_hi + 1 - seg_lo) / PB, (tile_upto + 1 - seg_lo) / PB - 2), nblk) : 0;
+    const int first_steady = max(all_lo - seg_lo + PB - 1, 0) / PB;
+    const int end_steady = __builtin_amdgcn_readfirstlane(all_hi >= seg_lo && tile_upto >= seg_lo ? min(min((all_hi + 1 - seg_lo) / PB, (tile_upto + 1 - seg_lo) / PB - 2), nblk) : 0);
     int k = 0;
-    for (; k < min(max(first_steady, first_whole - 2), nblk); ++k) step(std::false_type{}, k);
-    for (; k < end_steady && (hist & 0x33) == 0x33; ++k) step(std::true_type{}, k);
-    for (; k < nblk; ++k) step(std::false_type{}, k);
+    for (; k < min(max(first_steady, first_whole - 2), nblk); ++k) { step(std::false_type{}, k, scores, scores_next); scores = scores_next; }
+    for (; k + 1 < min(end_steady, clear - 2); k += 2) { step(std::true_type{}, k, scores, scores_next); step(std::true_type{}, k + 1, scores_next, scores); }
+    for (; k < nblk; ++k) { step(std::false_type{}, k, scores, scores_next); scores = scores_next; }
     brought<0>();                             // (what was asked for beyond the last block lands before the LDS is another workgroup's)
     again = *nan_flag != 0;
   }
