@@ -1659,11 +1659,25 @@ def decode_partitions_e4m3(num_seqs: int, Hq: int, Hkv: int, max_context: int, s
 
 
 def prompt_partitions_e4m3(tokens: int, num_seqs: int, Hq: int, Hkv: int, D: int, max_context: int, span: int = 0) -> tuple:
-    """(keys per partition, partitions) of a launch of prompt portions over an 8-bit cache, in tiles of 128 (token, head) pairs."""
+    """(keys per partition, partitions) of a launch of prompt portions over an 8-bit cache, in tiles of 128 (token, head) pairs.
+
+    A workgroup walks a range at 17 ns a key while most of them have a compute unit to themselves (up to 128), 22 ns up to 256, 27 ns two
+    to a unit, and in turns beyond 512; partial results of partitions are written and read at 4 TB/s, and joining them is a launch
+    of 5 us. The number of partitions that this makes cheapest, of at least 256 keys. 32 heads over 8 of 128: 489 tokens over
+    8,192 keys 135 us whole, 92 in 3, 82 in 4, 91 in 8; 256 over 32,256 keys 553 whole, 203 in 4, 138 in 8; 2,000 over 8,000 keys 222
+    whole, 247 in 2; 16 over 8: 2,048 tokens from the start 44 whole, 56 in 2."""
     G = Hq // Hkv
     keys = max(1, min(max_context, span + 128 // G + 64) if span else max_context)
-    groups = (tokens * G // 128 + 1) * Hkv
-    parts = max(1, min(-(-512 // groups), keys // 512))
+    tiles = max(1, tokens * G // 128) * Hkv
+    most, size = keys // 256, D / 128
+    best, parts = None, 1
+    for p in (1, 128 // tiles, 256 // tiles, 512 // tiles, 1024 // tiles) if tiles <= 512 and most > 1 else ():
+        p = max(1, min(p, most))
+        groups = tiles * p
+        walk = keys / p * size * (0.017 if groups <= 128 else 0.022 if groups <= 256 else 0.027 * max(1.0, groups / 512))
+        cost = walk if p == 1 else walk + 5 + tokens * Hq * p * (D + 2) * 8 / 4e6
+        if best is None or cost < best:
+            best, parts = cost, p
     if parts == 1:
         return 0, 1
     part = -(-keys // (parts * 64)) * 64
