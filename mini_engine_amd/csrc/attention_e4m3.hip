@@ -453,8 +453,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
   }
   const int q0 = a.cu[b], q_len = a.cu[b + 1] - q0;
   const int col0 = (tile - (int)((int64_t)q0 * a.G / COLS) - b) * COLS;
-  if (col0 >= q_len * a.G) return;
   const int L = context_of(a, b), start = L - q_len;
+  asm volatile("" ::"s"(L));                  // (asked for together with the counts)
+  if (col0 >= q_len * a.G) return;
   const int32_t* __restrict__ table = a.tables + (int64_t)b * a.table_stride;
   // the keys that the tile's columns see, and this segment's share of them
   const int last_tok = min(col0 + COLS, q_len * a.G) - 1;
@@ -470,48 +471,17 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
   const int64_t row = q0 + tok;
   float m = NONE, l = 0.f;
   const int lo = valid ? first_seen(a, max(start + tok, 0)) : 0, hi = valid ? start + tok : -1;      // the keys that the column sees
-  // The column's query as two e4m3 numbers each under one power, x = (high + low / 16) 2^p with |high| < 256: what rounding to high leaves of a
-  // bfloat16 has 4 bits, so the two are exact for numbers down to 2^-14 of the largest and off by 2^-22 of the largest below.
-  i32x8 q[CB];
-  uint32_t q_powers;                          // of high, of low; in the third byte, of high in the lower lanes and of low in the upper ones
+  uint4 raw[KC][4];                           // the column's query: channels 64 j + 32 h ..: a lane's 32; of an odd last 32 a lane has 16
   {
     const bf16_t* from = a.q + row * a.q_stride + (int64_t)head * HD;
-    uint4 raw[KC][4];                         // channels 64 j + 32 h ..: a lane's 32; of an odd last 32 a lane has 16
-    uint32_t top = 0;
 #pragma unroll
     for (int j = 0; j < KC; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         if (2 * j + 1 == CB && e >= 2) break;
         const int c = 64 * j + (2 * j + 1 < CB ? 32 : 16) * h + 8 * e;
-        uint4 x = *reinterpret_cast<const uint4*>(from + (c < HD ? c : 0));
-        if (!valid || c >= HD) x = make_uint4(0, 0, 0, 0);
-        raw[j][e] = x;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { const uint32_t w = (&x.x)[i]; top = max(top, max(w & 0x7fffu, (w >> 16) & 0x7fffu)); }
-      }
-    const auto both = __builtin_amdgcn_permlane32_swap(top, top, false, false);
-    const int power = min(max((int)(max(both[0], both[1]) >> 7) - 7, 4), 247);      // the largest number between 128 and 256 of it
-    const float down = __uint_as_float((uint32_t)(254 - power) << 23);
-    q_powers = (uint32_t)power | (uint32_t)(power - 4) << 8 | (uint32_t)(power - (h ? 4 : 0)) << 16;
-#pragma unroll
-    for (int j = 0; j < KC; ++j)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {           // four channels at a time
-        if (2 * j + 1 == CB && e >= 4) break;
-        const uint32_t w[2] = {(&raw[j][e >> 1].x)[2 * (e & 1)], (&raw[j][e >> 1].x)[2 * (e & 1) + 1]};
-        float x[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16) * down;
-        int high = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
-        high = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], high, true);
-        float r[4];
-        r[0] = (x[0] - __builtin_amdgcn_cvt_f32_fp8(high, 0)) * 16.f; r[1] = (x[1] - __builtin_amdgcn_cvt_f32_fp8(high, 1)) * 16.f;
-        r[2] = (x[2] - __builtin_amdgcn_cvt_f32_fp8(high, 2)) * 16.f; r[3] = (x[3] - __builtin_amdgcn_cvt_f32_fp8(high, 3)) * 16.f;
-        int low = __builtin_amdgcn_cvt_pk_fp8_f32(r[0], r[1], 0, false);
-        low = __builtin_amdgcn_cvt_pk_fp8_f32(r[2], r[3], low, true);
-        if (2 * j + 1 < CB) { q[2 * j][e] = high; q[(2 * j + 1) % CB][e] = low; }
-        else { q[2 * j][e] = high; q[2 * j][(4 + e) & 7] = low; }
+        raw[j][e] = *reinterpret_cast<const uint4*>(from + (c < HD ? c : 0));
+        if (!valid || c >= HD) raw[j][e] = make_uint4(0, 0, 0, 0);
       }
   }
   f32x16 acc[DC];
@@ -632,6 +602,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
           ka[j].half[e] = 16 * last < HD || 16 * piece < HD ? w : u32x4v{0, 0, 0, 0};
         }
     };
+    // The column's query as two e4m3 numbers each under one power, x = (high + low / 16) 2^p with |high| < 256: what rounding to high leaves of a
+    // bfloat16 has 4 bits, so the two are exact for numbers down to 2^-14 of the largest and off by 2^-22 of the largest below.
+    i32x8 q[CB];
+    uint32_t q_powers;                          // of high, of low; in the third byte, of high in the lower lanes and of low in the upper ones
     // product i of a tile of scores: high and low of 64 channels in turn, or both of 32 (a lane's power is for 32 of the 64 numbers: those in
     // the first four registers of both halves of the lanes, or those in the last four)
     uint32_t k_powers = 0;
@@ -649,6 +623,40 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
     // way, in this order, the keys and values of (3, 2), (4, 3), (5, 4).
     bring_keys(0, keys_of(0)); bring_keys(1, keys_of(1)); bring_values(0, values_of(0)); bring_values(1, values_of(1)); bring_keys(2, keys_of(2));
     bring_keys(3, keys_of(3)); bring_values(2, values_of(2)); bring_values(3, values_of(3));
+    {
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < KC; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (2 * j + 1 == CB && e >= 2) break;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) { const uint32_t w = (&raw[j][e].x)[i]; top = max(top, max(w & 0x7fffu, (w >> 16) & 0x7fffu)); }
+        }
+      const auto both = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+      const int power = min(max((int)(max(both[0], both[1]) >> 7) - 7, 4), 247);      // the largest number between 128 and 256 of it
+      const float down = __uint_as_float((uint32_t)(254 - power) << 23);
+      q_powers = (uint32_t)power | (uint32_t)(power - 4) << 8 | (uint32_t)(power - (h ? 4 : 0)) << 16;
+#pragma unroll
+      for (int j = 0; j < KC; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {           // four channels at a time
+          if (2 * j + 1 == CB && e >= 4) break;
+          const uint32_t w[2] = {(&raw[j][e >> 1].x)[2 * (e & 1)], (&raw[j][e >> 1].x)[2 * (e & 1) + 1]};
+          float x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16) * down;
+          int high = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+          high = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], high, true);
+          float r[4];
+          r[0] = (x[0] - __builtin_amdgcn_cvt_f32_fp8(high, 0)) * 16.f; r[1] = (x[1] - __builtin_amdgcn_cvt_f32_fp8(high, 1)) * 16.f;
+          r[2] = (x[2] - __builtin_amdgcn_cvt_f32_fp8(high, 2)) * 16.f; r[3] = (x[3] - __builtin_amdgcn_cvt_f32_fp8(high, 3)) * 16.f;
+          int low = __builtin_amdgcn_cvt_pk_fp8_f32(r[0], r[1], 0, false);
+          low = __builtin_amdgcn_cvt_pk_fp8_f32(r[2], r[3], low, true);
+          if (2 * j + 1 < CB) { q[2 * j][e] = high; q[(2 * j + 1) % CB][e] = low; }
+          else { q[2 * j][e] = high; q[2 * j][(4 + e) & 7] = low; }
+        }
+    }
     step_barrier();                           // (the flag)
     brought<3 * PIECES>();
 #pragma unroll
@@ -828,41 +836,49 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
 }
 
 // Joins the partitions of a (row, head): out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p. A wave to a (row, head): a lane weighs a
-// partition, then all of them sum the channels, eight partitions asked for at a time. DECODE: row t is request t, which may have fewer.
+// partition, then all of them sum the channels, eight partitions asked for at a time, the first eight before anything else is known.
+// DECODE: row t is request t, which may have fewer partitions than there is room for; what lies behind them is read and not used.
 template <bool DECODE>
 __global__ void __launch_bounds__(256) attn8_join_kernel(Attn8Args a, int64_t rows) {
   const int lane = threadIdx.x & 63;
   const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (at >= rows * a.Hq) return;
-  const int64_t t = at / a.Hq;
-  const int head = (int)(at - t * a.Hq);
-  const int parts = DECODE ? parts_of(a, context_of(a, (int)t)) : a.num_parts;
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + at * a.num_parts;
   const float* po = a.part_o + at * a.num_parts * HD;
   constexpr int CH = (HD + 63) / 64;
-  float M = NONE;
-  for (int p = lane; p < parts; p += 64) M = fmaxf(M, ml[p].x);
+  float v[8][CH];
+  auto ask = [&](int p) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+#pragma unroll
+      for (int j = 0; j < CH; ++j) {
+        const int d = lane + 64 * j;
+        v[e][j] = po[(int64_t)min(p + e, a.num_parts - 1) * HD + (HD % 64 == 0 || d < HD ? d : 0)];
+      }
+  };
+  ask(0);
+  const float2 none = make_float2(NONE, 0.f);
+  float2 mine = lane < a.num_parts ? ml[lane] : none;
+  const int64_t t = at / a.Hq;
+  const int head = (int)(at - t * a.Hq);
+  const int parts = DECODE ? parts_of(a, context_of(a, (int)t)) : a.num_parts;
+  if (lane >= parts) mine = none;
+  float M = mine.x;
+  for (int p = lane + 64; p < parts; p += 64) M = fmaxf(M, ml[p].x);
   M = wave_max(M);
   float sum = 0.f, o[CH];
 #pragma unroll
   for (int j = 0; j < CH; ++j) o[j] = 0.f;
   for (int p0 = 0; p0 < parts; p0 += 64) {
-    const float2 mine = p0 + lane < parts ? ml[p0 + lane] : make_float2(NONE, 0.f);
+    if (p0 > 0) mine = p0 + lane < parts ? ml[p0 + lane] : none;
     const float f = mine.y == 0.f ? 0.f : exp2f(mine.x - M);      // (no key: nothing, whatever the maxima)
     sum += wave_sum(f * mine.y);
     const int upto = min(64, parts - p0);
     for (int i = 0; i < upto; i += 8) {
-      float v[8][CH];
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-#pragma unroll
-        for (int j = 0; j < CH; ++j) {
-          const int d = lane + 64 * j;
-          v[e][j] = po[(int64_t)(p0 + min(i + e, upto - 1)) * HD + (HD % 64 == 0 || d < HD ? d : 0)];
-        }
+      if (p0 + i > 0) ask(p0 + i);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float fe = i + e < upto ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), i + e)) : 0.f;
+        const float fe = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), i + e));
 #pragma unroll
         for (int j = 0; j < CH; ++j) o[j] = i + e < upto ? fmaf(fe, v[e][j], o[j]) : o[j];
       }
