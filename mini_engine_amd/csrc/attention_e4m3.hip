@@ -4,16 +4,19 @@
 //   o = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q . k_j),  over the keys j that the query sees; a sink adds exp(sink) to
 //   the denominator.
 //
-// The stored numbers times their power are bfloat16 numbers, so they are turned into such (v_cvt_scalef32_pk_bf16_fp8: two numbers and
-// the power in one instruction, exactly) and both products run on v_mfma_f32_16x16x32_bf16 without a rounding that a bfloat16 cache would not
-// have. Everything is computed transposed, as S^T = K Q^T and O^T += V^T P^T, over blocks of 64 keys; a "column" is one (query
-// token, query head) pair of a key head. With n = lane & 15, g = lane >> 4:
+// Everything is computed transposed, as S^T = K Q^T and O^T += V^T P^T; a "column" is one (query token, query head) pair of a key head.
+// Maxima, sums and accumulators are float32 and per column; probabilities are rounded to bfloat16 for the second product, as they are
+// over a bfloat16 cache.
+//
+// The stored numbers times their power are bfloat16 numbers: what the products take turned into such is turned exactly
+// (v_cvt_scalef32_pk_bf16_fp8, two numbers and the power in one instruction). So it is for single tokens, where both products run on
+// v_mfma_f32_16x16x32_bf16 over blocks of 64 keys. With n = lane & 15, g = lane >> 4:
 //   * the four tiles of S^T let row m of tile tt stand for key 16 (m / 4) + 4 tt + m % 4, so lane (n, g) ends with the 16 keys
 //     16 g .. 16 g + 15 of column n in order: the operand of the second product, without a movement of data;
 //   * a lane reads 16 bytes of keys (16 channels 64 j + 16 g ..) and of values (16 keys 16 g .. of channel 16 dt + n) at a time: two
 //     products' operands each. Which channel lies in which slot of the first product is free as long as the queries follow;
 //   * every lane's keys of a block lie under one power, and so do its values: one byte and a shift per lane.
-// Maxima, sums and accumulators are float32 and per column.
+// Prompts are described at their kernel.
 //
 // Keys that a column does not see are replaced, never multiplied by zero: scores by "none", stored values by zero bytes where no
 // column sees them; and where some columns of a prompt's tile see a key whose value is NaN and others do not, the tile's columns are done
@@ -139,7 +142,7 @@ __device__ __forceinline__ void load_values(const Attn8Args& a, const Pages& p, 
   b.vcode = a.v_powers[(at << (a.page_shift - 4)) + (off >> 4)];
 }
 
-// The queries of one column, in the order of the channels that load_block gives a lane.
+// The queries of one column, in the order of the channels that load_keys gives a lane.
 __device__ __forceinline__ void load_q(const bf16_t* row, bool valid, int g, bf16x8 (&q)[2 * KL]) {
 #pragma unroll
   for (int j = 0; j < KL; ++j)
@@ -166,60 +169,58 @@ __device__ __forceinline__ void hide_values(Block& b, int t0, int lo, int L, int
   }
 }
 
-template <int CT>
-struct Columns {
-  int lo[CT], hi[CT];            // keys [lo, hi] that the column sees (hi < lo: none)
-  float m[CT], l[CT];            // reference point of the exponentials (log2 domain), this lane's share of the sum
-  f32x4 acc[CT][DT];
+struct Column {
+  int lo, hi;                    // keys [lo, hi] that the column sees (hi < lo: none)
+  float m, l;                    // reference point of the exponentials (log2 domain), this lane's share of the sum
+  f32x4 acc[DT];
 };
 
-// The softmax of N tiles of scores (4 N keys of a lane, from `first` on) in column tile ct: under the column's reference point, which
-// rises where it must (the column's sums with it), their probabilities are added to the sum and rounded to bfloat16 as the second
-// product's operand (the sum takes them unrounded). FULL: the column sees all keys; else `seen` gets the bits of the lane's keys that
-// it does. there: they lie in a page.
-template <int CT, bool FULL, int N>
-__device__ __forceinline__ void softmax_tiles(const f32x4* st, float sc, int first, bool there, int ct, Columns<CT>& c, uint32_t& seen, bf16x8* pb) {
-  float s[4 * N];
+// The softmax of a block's scores (16 keys of a lane, from `first` on): under the column's reference point, which rises where it must (the
+// column's sums with it), their probabilities are added to the sum and rounded to bfloat16 as the second product's operand (the sum
+// takes them unrounded). FULL: the column sees all keys. there: they lie in a page.
+template <bool FULL>
+__device__ __forceinline__ void softmax(const f32x4 (&st)[4], float sc, int first, bool there, Column& c, bf16x8 (&pb)[2]) {
+  float s[16];
   float top = NONE;
+  uint32_t seen = 0;
   if constexpr (!FULL) {
-    const int from = max(c.lo[ct] - first, 0), to = min(c.hi[ct] - first, 4 * N - 1);
-    seen = there && to >= from && from < 4 * N ? (2u << to) - (1u << from) : 0u;
+    const int from = max(c.lo - first, 0), to = min(c.hi - first, 15);
+    seen = there && to >= from && from < 16 ? (2u << to) - (1u << from) : 0u;
   }
 #pragma unroll
-  for (int i = 0; i < 4 * N; ++i) {
-    s[i] = st[i >> 2][i & 3];
+  for (int i = 0; i < 16; ++i) {
+    s[i] = st[i >> 2][i & 3] * sc;
     if constexpr (!FULL) s[i] = (seen >> i) & 1 ? s[i] : NONE;
     top = fmaxf(top, s[i]);
   }
-  if (__any(top > 0.5f * NONE && top * sc > c.m[ct] + RESCALE_STEP)) {
-    top = max_of_column(top);
-    const float next = top > 0.5f * NONE ? top * sc : NONE;
-    if (next > c.m[ct] + RESCALE_STEP) {
-      const float f = __builtin_amdgcn_exp2f(c.m[ct] - next);
-      c.l[ct] *= f;
+  if (__any(top > c.m + RESCALE_STEP)) {
+    const float next = max_of_column(top);
+    if (next > c.m + RESCALE_STEP) {
+      const float f = __builtin_amdgcn_exp2f(c.m - next);
+      c.l *= f;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c.acc[ct][dt][i] *= f;
-      c.m[ct] = next;
+        for (int i = 0; i < 4; ++i) c.acc[dt][i] *= f;
+      c.m = next;
     }
   }
   float sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4 * N; ++i) {
-    float p = __builtin_amdgcn_exp2f(fmaf(s[i], sc, -c.m[ct]));
+  for (int i = 0; i < 16; ++i) {
+    float p = __builtin_amdgcn_exp2f(s[i] - c.m);
     if constexpr (!FULL) p = (seen >> i) & 1 ? p : 0.f;      // while a column has seen no key, its reference point is NONE too
     sum += p;
     pb[i >> 3][i & 7] = static_cast<bf16_t>(p);
   }
-  c.l[ct] += sum;
+  c.l += sum;
 }
 
 // One block out of registers, for a wave's single column tile; more_keys and more_values ask for the next one's, each as soon as this one's
 // have been used, into the same registers. FULL: every column sees every key of it, and all of them lie in pages. (Otherwise all columns
 // see the same keys: what none of them sees is zeroed, and a NaN among the others is everybody's.)
 template <bool FULL, typename K, typename V>
-__device__ __forceinline__ void attend(const Attn8Args& a, Block& b, int t0, int lo, int L, int g, const bf16x8 (&q)[2 * KL], Columns<1>& c, K more_keys,
+__device__ __forceinline__ void attend(const Attn8Args& a, Block& b, int t0, int lo, int L, int g, const bf16x8 (&q)[2 * KL], Column& c, K more_keys,
                                        V more_values) {
   const float kpow = power_of(b.kcode), vpow = power_of(b.vcode);
   f32x4 st[4];
@@ -238,14 +239,13 @@ __device__ __forceinline__ void attend(const Attn8Args& a, Block& b, int t0, int
   }
   more_keys();
   bf16x8 pb[2];
-  uint32_t seen;
-  softmax_tiles<1, FULL, 4>(st, a.scale * LOG2E, t0 + 16 * g, b.there, 0, c, seen, pb);
+  softmax<FULL>(st, a.scale * LOG2E, t0 + 16 * g, b.there, c, pb);
   if constexpr (!FULL) hide_values(b, t0, lo, L, g);
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-      c.acc[0][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(b.v[dt][2 * h], b.v[dt][2 * h + 1], vpow), pb[h], c.acc[0][dt], 0, 0, 0);
+      c.acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(b.v[dt][2 * h], b.v[dt][2 * h + 1], vpow), pb[h], c.acc[dt], 0, 0, 0);
   more_values();
 }
 
@@ -283,11 +283,11 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attn8_decode_kernel(At
   const bool valid = n < ncols;
   const int head = kvh * a.G + ctile * 16 + (valid ? n : 0);
   const int32_t* __restrict__ table = a.tables + (int64_t)b * a.table_stride;
-  Columns<1> c;
-  c.m[0] = NONE; c.l[0] = 0.f;
-  c.lo[0] = lo; c.hi[0] = valid ? pos : -1;
+  Column c;
+  c.m = NONE; c.l = 0.f;
+  c.lo = lo; c.hi = valid ? pos : -1;
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) c.acc[0][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int dt = 0; dt < DT; ++dt) c.acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   int t0 = p_lo + BK * wave;
   if (t0 < p_hi) {
     constexpr int STEP = 4 * BK;
@@ -310,15 +310,15 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attn8_decode_kernel(At
       t0 += STEP;
     }
   }
-  const float l = sum_of_column(c.l[0]);
+  const float l = sum_of_column(c.l);
   const int stride = HD + 2;
   if (valid) {
     float* mine = lds + (wave * ncols + n) * stride;
-    if (g == 0) { mine[HD] = c.m[0]; mine[HD + 1] = l; }
+    if (g == 0) { mine[HD] = c.m; mine[HD + 1] = l; }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) mine[16 * dt + 4 * g + i] = c.acc[0][dt][i];
+      for (int i = 0; i < 4; ++i) mine[16 * dt + 4 * g + i] = c.acc[dt][i];
   }
   __syncthreads();
   for (int e = threadIdx.x; e < ncols * HD; e += 256) {
@@ -346,21 +346,30 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attn8_decode_kernel(At
 
 // =====================================================================================
 // Portions of prompts. A tile is 128 columns of one request and key head; each of the 4 waves of its workgroup has 32 of them, a column to
-// two lanes (l and l ^ 32). The workgroup walks the keys that its columns see in blocks of 32 with v_mfma_f32_32x32x16_bf16 (half as many
-// instructions as tiles of 16 x 16 take, and one column's state to a lane instead of two). Row r of a tile of scores stands for the key whose bits 2
-// and 3 are exchanged: lane l then holds keys 8 h .. 8 h + 7 and 16 + 8 h .. of its column (h = l / 32), the values' operand as it is.
-// A block's bytes go to LDS by themselves (global_load_lds_dwordx4), five and six blocks ahead, and are turned into bfloat16 once, two and
-// three blocks ahead, from which every wave reads its operands (each wave all conversions for itself would be a third of its vector instructions; bytes
-// held in registers could be asked for one step ahead only, less than a trip to memory). What a wave brings of a block lies in one page
-// under one power, so pages, powers and addresses are scalars, and a lane turns into bfloat16 what it has brought itself.
-//   keys    [pieces of 8 channels][32 rows] of 16 bytes: a read of 16 bytes a lane is worked off for lanes 0-3, 12-15 and 20-27 together,
-//           then for the others of 32, which so lie in 16 different groups of banks. A wave writes two fours of a piece's rows; their fours
-//           change places in every second pair of pieces (row ^ 4), which spreads the writes over all banks and leaves the reads as they are.
+// two lanes (l and l ^ 32). The workgroup walks the keys that its columns see in blocks of 32, which half as many instructions take as
+// tiles of 16 x 16, with one column's state to a lane instead of two. Row r of a tile of scores stands for the key whose bits 2 and 3 are
+// exchanged: lane l then holds keys 8 h .. 8 h + 7 and 16 + 8 h .. of its column (h = l / 32), the values' operand as it is.
+//   scores  v_mfma_scale_f32_32x32x64_f8f6f4 takes the cached bytes as they are and a block's power as the product's own. The query is two
+//           e4m3 numbers (below), so a tile takes as long as in bfloat16 (twice the products at twice the rate), without turning keys
+//           into anything, and half the bytes of keys out of LDS: 8,192 tokens, 32 heads over 8 of 128, 554 -> 518 us.
+//   values  are turned into bfloat16 once, two blocks ahead, from which every wave reads its operands of v_mfma_f32_32x32x16_bf16.
+// A block's bytes go to LDS by themselves (global_load_lds_dwordx4), five and six blocks ahead (bytes held in registers could be asked for one
+// step ahead only, less than a trip to memory). What a wave brings of a block lies in one page under one power, so pages, powers and
+// addresses are scalars, found for 32 blocks at a time, and a lane turns into bfloat16 what it has brought itself.
+//   keys    [4 waves' 8 keys][16 channels][8 keys] of 16 bytes, the second 16 keys 128 bytes further on: a read of 16 bytes a lane is
+//           worked off for lanes 0-3, 12-15 and 20-27 together, then for the others of 32, which so lie in 16 different groups of banks.
 //   values  [8 keys][channel] of 16 bytes.
 // Step k of the walk is a pipeline: beside the numbers of block k's softmax the products of block k + 1's scores, beside the products of
-// its values the conversion of block k + 2's values and block k + 3's keys and the reads of block k + 2's keys (read in front of their
-// products instead, behind the barrier, every step began with a wait for LDS). One barrier a step. LDS: bytes of four blocks, keys of two,
-// values of three.
+// its values the conversion of block k + 2's values and the reads of its keys. One barrier a step. LDS: bytes of keys of eight blocks, of
+// values of four, values of three. Weights are taken under the reference point as it is, and only where their sum says that the maximum has
+// risen by much once more: the maximum of every block (11 instructions a step of 80, and exponentials that wait for it) and a sum of
+// single weights instead of pairs cost 6%; registers of scores that change their meaning every second step instead of being copied, 2%.
+//
+// Bound by the matrix cores' and the vector units' shared issue: of 930 cycles a step and wave at 8,192 tokens 512 are products (55% of the
+// time; two waves to a unit) and 45% of a wave's time is issue. 470 us there are 1,170 TF/s, against 1,430 of a large bfloat16 product.
+// A workgroup alone on its unit takes 0.5 us a step, two of them 0.9, so a short prompt takes what its last tile takes: 2,048 tokens (16
+// heads over 8) 44 us, of which 5.5 until the first step. Two sets of 4 waves that share a tile's keys came to 41 us there and
+// cost portions of few tokens 3 us; 64 columns to a wave left one wave to a unit: 657 us for 590.
 // Grid (tiles x key heads, segments): surplus tiles (the grid is made for the most there can be) exit.
 // =====================================================================================
 typedef float f32x16 __attribute__((ext_vector_type(16)));
