@@ -201,9 +201,10 @@ def attend(q, numbers, step: Step, scale, Hq, Hkv, window=None, chunk=None, sink
 
 def attention_bound(o, spread):
     """What the kernels may be off: the result is rounded to bfloat16 (2^-8 of it), and so is every probability before it
-    multiplies its value while the sum takes it unrounded (2^-8 of the values' weighted sizes). Sums, scores and exponentials are float32:
-    a score is off by about 1e-6 of what its products add up to, some tens, and so is a probability relative to itself, 1e-4 in all."""
-    return 2.0 ** -8 * o.abs() + (2.0 ** -8 + 2e-4) * spread + 1e-30
+    multiplies its value (2^-8 of the values' weighted sizes; where the sum takes the rounded ones too, sum_j p_j e_j (v_j - o) with
+    |e_j| <= 2^-8 instead of sum_j p_j e_j v_j: another 2^-8 of the result at most). Sums, scores and exponentials are float32: a score is
+    off by about 1e-6 of what its products add up to, some tens, and so is a probability relative to itself, 1e-4 in all."""
+    return 2.0 ** -7 * o.abs() + (2.0 ** -8 + 2e-4) * spread + 1e-30
 
 
 def place_bound(exact, powers):

@@ -215,12 +215,12 @@ def _attention(q, pages, step, scale, Hq, Hkv, D, window=None, chunk=None, sinks
                                     step.decode_context, scale, window, Hq, Hkv, D, max_prefill_context=step.prefill_context, chunk=chunk, sinks=on(sinks))
 
 
-def _check_attention(lengths, Hq, Hkv, D, page, seed=0, gap=0, pages=None, loud=1.0, **options):
+def _check_attention(lengths, Hq, Hkv, D, page, seed=0, gap=0, pages=None, loud=1.0, scale=None, **options):
     gen = _gen(seed)
     step = Step(lengths, page, gen)
     pages = mild_pages(step.pages, Hkv, D, page, gen) if pages is None else pages(step, gen)
     q = (loud * torch.randn(step.T, Hq * D + gap, generator=gen)).to(torch.bfloat16)
-    scale = D ** -0.5
+    scale = D ** -0.5 if scale is None else scale
     got = _attention(q.to(DEV)[:, :Hq * D], pages, step, scale, Hq, Hkv, D, **options)
     o, spread = attend(q[:, :Hq * D].double().view(step.T, Hq, D), PlainPages.of(pages).numbers(), step, scale, Hq, Hkv, **options)
     got = got.cpu().double().view(step.T, Hq, D)
@@ -267,6 +267,51 @@ def test_attention_long(lengths, window):
 def test_attention_uneven_scores():
     """Loud queries: a few keys have all of the softmax, and the maximum rises again and again."""
     got, o, _ = _check_attention(MIX + [(200, 900)], 4, 2, 64, 16, seed=3, loud=20.0)
+
+
+@pytest.mark.parametrize("scale", [-0.2, 0.0, float("nan")])
+@pytest.mark.parametrize("lengths", [[(1, 40)], [(20, 40)]])
+def test_attention_scales_that_are_refused(scale, lengths):
+    """As over a cache of the activations' type: scales are positive."""
+    with pytest.raises(ops.KernelError, match="scale must be positive"):
+        _check_attention(lengths, 4, 2, 64, 16, seed=9, scale=scale)
+
+
+def test_attention_of_a_small_scale():
+    """Every key counts nearly alike."""
+    _check_attention(MIX + [(200, 900)], 4, 2, 64, 16, seed=9, scale=1e-3, loud=4.0)
+
+
+@pytest.mark.parametrize("D", [16, 80, 128, 256])
+def test_attention_queries_of_all_sizes(D):
+    """Channels of very different sizes, rows of zeros; and a power of two that moves from the scale to the queries changes no bit."""
+    gen = _gen(D)
+    step = Step(MIX + [(200, 900)], 16, gen)
+    pages = mild_pages(step.pages, 2, D, 16, gen)
+    q = torch.randn(step.T, 4, D, generator=gen) * torch.exp2(-(torch.arange(D) % 23).float())
+    q[::5, 1] = 0.0
+    q = q.to(torch.bfloat16).view(step.T, 4 * D)
+    got = _attention(q.to(DEV), pages, step, 0.25, 4, 2, D)
+    o, spread = attend(q.double().view(step.T, 4, D), PlainPages.of(pages).numbers(), step, 0.25, 4, 2)
+    assert ((got.cpu().double().view(step.T, 4, D) - o).abs() <= attention_bound(o, spread)).all()
+    for power in (-60, 60):
+        moved = _attention((q.float() * 2.0 ** power).to(torch.bfloat16).to(DEV), pages, step, 0.25 * 2.0 ** -power, 4, 2, D)
+        assert torch.equal(moved, got)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("D", [48, 128])
+def test_attention_a_query_that_is_no_number(D, bad):
+    """It makes NaN of its row and head and of nothing else."""
+    gen = _gen(12)
+    step = Step([(1, 300), (1, 700), (40, 0), (130, 400)], 16, gen)
+    pages = mild_pages(step.pages, 2, D, 16, gen)
+    q = torch.randn(step.T, 4, D, generator=gen).to(torch.bfloat16)
+    rows = [1, 41, 42, step.T - 1]
+    for r in rows:
+        q[r, 2, 5] = bad
+    got = torch.isnan(_attention(q.view(step.T, 4 * D).to(DEV), pages, step, 0.2, 4, 2, D).cpu().view(step.T, 4, D))
+    assert got[rows, 2].all() and int(got.sum()) == len(rows) * D
 
 
 @pytest.mark.parametrize("D", [32, 128, 256])
