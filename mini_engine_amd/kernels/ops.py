@@ -703,7 +703,7 @@ class HipBackend:
         at its place 0 opens it anew, any other keeps what stands in front of its first place: the power never falls, and where it
         grows those numbers are rounded again (exactly, unless they fall below e4m3's smallest normal number). Places behind the last
         one written hold nothing: they keep their bytes, which a grown power leaves without meaning. Rows of one block that follow each
-        other in another order are taken as calls one after the other; a block whose rows stand apart in one call holds either of them.
+        other in another order are taken as calls one after the other; what a block holds whose rows stand apart in one call is not defined.
         slots below 0 or beyond the pages are skipped. (reference models/qwen3.py:34-36, layers/rotary_embedding.py:20-25,
         csrc/kv_cache.cu:10-31, whose cache has the activations' type.)"""
         what = "qk_norm_rope_store_e4m3"          # (messages are formed where they are needed)
@@ -745,6 +745,8 @@ class HipBackend:
         a power of two from 16 on. Returns [T, Hq*D]. (reference layers/attention.py:63-76, over a cache of the activations' type.)"""
         what = "paged_attention_e4m3"
         T, B = q.shape[0], context_lens.numel()
+        if not (Hkv >= 1 and Hq >= 1 and Hq % Hkv == 0):
+            raise KernelError(f"{what}: {Hq} query heads are no multiple of {Hkv} key heads")
         if q.dtype != torch.bfloat16:
             raise KernelError(f"{what}: queries must be bfloat16, got {q.dtype}")
         if not (q.dim() == 2 and q.shape[1] == Hq * D and q.stride(1) == 1 and (T <= 1 or q.stride(0) >= Hq * D)):

@@ -115,6 +115,9 @@ def test_attention_refusals():
     _refused(call, a, "prefill_cu", num_decodes=3)
     _refused(call, a, "power of two", page=8)
     _refused(call, a, "pages must be", Hkv=4)
+    _refused(call, a, "no multiple", Hkv=0)
+    _refused(call, a, "no multiple", Hkv=8, window=4)
+    _refused(call, a, "no multiple", Hkv=3)
 
 
 def test_libraries_of_other_head_sizes_are_refused():
