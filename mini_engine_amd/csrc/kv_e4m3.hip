@@ -1,6 +1,6 @@
 // The write into the 8-bit cache (e4m3.h): per-head RMSNorm of q and k, rotation, and the scatter of k and v into their pages, in
 // one launch over the packed rows. q goes out as rows of its own, rounded to bfloat16 once; k and v are rounded to e4m3 once, from
-// the float32 results.
+// the float32 results, and from exact ones where that could make a difference.
 //
 //   k' = rotated(w * k / rms(k));  block (16 places of a page, head): p = max(p_before if places in front of the call's first
 //   place are held, least power with max |k'| <= 448 * 2^p);  stored: e4m3(k' 2^-p), numbers held before: e4m3(old 2^(p_before - p)).
@@ -106,6 +106,65 @@ __device__ __forceinline__ void norm_rotate(const AppendArgs& a, bool norm, cons
   }
 }
 
+// The same exactly, as far as a rounding to 4 significant bits can see: sum and root in double, products and their sums as the rounded
+// number and what it leaves (by fma, and by the sums' own errors, after Dekker and Knuth), and the result rounded to the odd neighbour
+// where it is none: the rounding to come then goes as that of the exact number would.
+struct Pair { float hi, lo; };
+__device__ __forceinline__ Pair sum_of(float a, float b) {
+#pragma clang fp contract(off)
+  const float s = a + b, t = s - a;
+  return Pair{s, (a - (s - t)) + (b - t)};
+}
+__device__ __forceinline__ float odd(Pair x) {
+  const uint32_t bits = __float_as_uint(x.hi);
+  const bool moves = x.lo != 0.f && !(bits & 1) && (bits << 1) - 1 < 0xfeffffffu;      // (neither zero nor infinite nor NaN)
+  return __uint_as_float(moves ? ((x.lo > 0.f) == (x.hi > 0.f) ? bits + 1 : bits - 1) : bits);
+}
+template <int L2>
+__device__ __forceinline__ void norm_rotate_key(const AppendArgs& a, bool norm, const Weights& w, const Turn& t, bf16x8 raw1, bf16x8 raw2, bool there, float (&y1)[8],
+                                                float (&y2)[8]) {
+#pragma clang fp contract(off)
+  Pair inv = {1.f, 0.f};
+  if (norm) {
+    double ss = 0.;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const double u = there ? static_cast<float>(raw1[i]) : 0.f, v = there ? static_cast<float>(raw2[i]) : 0.f;
+      ss = fma(u, u, fma(v, v, ss));
+    }
+#pragma unroll
+    for (int off = L2 / 2; off > 0; off >>= 1) ss += __shfl_xor(ss, off, ME_WAVE);
+    const double root = rsqrt(ss / (double)a.D + (double)a.eps);
+    inv.hi = (float)root;
+    inv.lo = (float)(root - (double)inv.hi);
+  }
+  auto normed = [&](float x, float weight) {
+    if (!norm) return Pair{x, 0.f};
+    const float m = inv.hi * weight, y = x * m;
+    return Pair{y, fmaf(x, m, -y) + x * fmaf(inv.lo, weight, fmaf(inv.hi, weight, -m))};
+  };
+  auto product = [](Pair x, float c) {
+    const float y = x.hi * c;
+    return Pair{y, fmaf(x.lo, c, fmaf(x.hi, c, -y))};
+  };
+  auto sum = [](Pair x, Pair y) {
+    const Pair s = sum_of(x.hi, y.hi);
+    return sum_of(s.hi, s.lo + (x.lo + y.lo));
+  };
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const Pair u = normed(there ? static_cast<float>(raw1[i]) : 0.f, w.w1[i]), v = normed(there ? static_cast<float>(raw2[i]) : 0.f, w.w2[i]);
+    if (a.table) {
+      const float c = i < 4 ? t.c0[2 * i] : t.c1[2 * i - 8], s = i < 4 ? t.c0[2 * i + 1] : t.c1[2 * i - 7];
+      y1[i] = odd(sum(product(u, c), product(v, -s)));
+      y2[i] = odd(sum(product(v, c), product(u, s)));
+    } else {
+      y1[i] = odd(u);
+      y2[i] = odd(v);
+    }
+  }
+}
+
 __device__ __forceinline__ int row_position(const AppendArgs& a, int64_t t) {
   return a.table ? min(max(a.positions[min(t, a.T - 1)], 0), a.table_positions - 1) : 0;
 }
@@ -113,6 +172,12 @@ __device__ __forceinline__ int row_slot(const AppendArgs& a, int64_t t) {
   const int s = t >= 0 && t < a.T ? a.slots[t] : -1;
   return s < a.slot_end ? s : -1;
 }
+
+// Whether a number, scaled for its block, lies so near to the middle between two e4m3 numbers that float32 may have put it on the other side:
+// within 8 of its steps. There it would be off by a whole step of e4m3 (one number in 650,000 was, most of them by one of the large
+// steps; what cancellation leaves further off is small, and so are its steps); one in 65,000 is done again by norm_rotate_key. 60 rows
+// of one token 6.4 us in float32 alone, 8.4 so; 7,900 rows of 32 and 8 heads of 128 48.5 and 51, with every key done so 59, all in double 66.
+__device__ __forceinline__ bool between(float x) { return ((__float_as_uint(x) + 0x80008u) & 0xfffffu) < 0x10u; }
 
 // The cnt rows from r on, of one block, of one key head (at most 16, ascending slots). Lane i holds the slot and the position of row r + i
 // (i < 16): everything else is asked for at once.
@@ -127,20 +192,19 @@ __device__ __forceinline__ void store_keys(const AppendArgs& a, int64_t r, int c
   uint8_t* code = a.k_powers + ((pg * a.Hkv + kvh) << (a.page_shift - 4)) + (in_page >> 4);
   const int before = begin > 0 ? min((int)*code - E4_BIAS, E4_MOST) : E4_LEAST;
   bf16x8 raw1[PASSES], raw2[PASSES];
-  int off[PASSES];
   Turn turn[PASSES];
   Weights w;
   const int at = active ? 8 * l : 0;
+  auto row_of = [&](int p) { return min(p * TOKENS + lane / L2, cnt - 1); };      // (beyond the run its last one: it changes no maximum)
+  auto load = [&](int p, bf16x8& x1, bf16x8& x2, Turn& t) {
+    const bf16_t* row = a.rows + (r + row_of(p)) * a.row_stride + (int64_t)(a.Hq + kvh) * a.D + at;
+    x1 = load8(row, a.wide); x2 = load8(row + half, a.wide);
+    load_turn(a, at, __shfl(positions, row_of(p)), t);
+  };
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
-    // (rows beyond the run repeat its last one: they change no maximum)
-    const int i = p * TOKENS + lane / L2, j = min(i, cnt - 1);
-    const int slot = __shfl(slots, j), position = __shfl(positions, j);
-    off[p] = i < cnt ? slot & (a.page - 1) : -1;
     if (p > 0 && p * TOKENS >= cnt) continue;      // (a single token is one pass)
-    const bf16_t* row = a.rows + (r + j) * a.row_stride + (int64_t)(a.Hq + kvh) * a.D + at;
-    raw1[p] = load8(row, a.wide); raw2[p] = load8(row + half, a.wide);
-    load_turn(a, at, position, turn[p]);
+    load(p, raw1[p], raw2[p], turn[p]);
   }
   load_weights(a, a.k_w, at, w);
   float x1[PASSES][8], x2[PASSES][8];
@@ -162,10 +226,27 @@ __device__ __forceinline__ void store_keys(const AppendArgs& a, int64_t r, int c
   const float scale = e4_pow2(-power);
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
-    if (!active || off[p] < 0) continue;
-    uint8_t* dst = base + (int64_t)(off[p] & (E4_BLOCK - 1)) * a.D + 8 * l;
+    if (p > 0 && p * TOKENS >= cnt) continue;
+    bool near = false;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) { x1[p][j] = e4_scaled(x1[p][j], scale); x2[p][j] = e4_scaled(x2[p][j], scale); }
+    for (int j = 0; j < 8; ++j) {
+      x1[p][j] = e4_scaled(x1[p][j], scale); x2[p][j] = e4_scaled(x2[p][j], scale);
+      near |= between(x1[p][j]) | between(x2[p][j]);
+    }
+    if (__builtin_expect(__any(near), 0)) {        // everything once more, asked for again (held until here, it would cost the queries' waves their registers)
+      asm volatile("" ::: "memory");
+      bf16x8 again1, again2;
+      Turn t;
+      Weights again;
+      load(p, again1, again2, t);
+      load_weights(a, a.k_w, at, again);
+      norm_rotate_key<L2>(a, a.k_w != nullptr, again, t, again1, again2, active, x1[p], x2[p]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) { x1[p][j] = e4_scaled(x1[p][j], scale); x2[p][j] = e4_scaled(x2[p][j], scale); }
+    }
+    const int place = __shfl(slots, row_of(p)) & (E4_BLOCK - 1);
+    if (!active || p * TOKENS + lane / L2 >= cnt) continue;
+    uint8_t* dst = base + (int64_t)place * a.D + 8 * l;
     *reinterpret_cast<u32x2*>(dst) = u32x2{e4_pack(x1[p][0], x1[p][1], x1[p][2], x1[p][3]), e4_pack(x1[p][4], x1[p][5], x1[p][6], x1[p][7])};
     *reinterpret_cast<u32x2*>(dst + half) = u32x2{e4_pack(x2[p][0], x2[p][1], x2[p][2], x2[p][3]), e4_pack(x2[p][4], x2[p][5], x2[p][6], x2[p][7])};
   }
@@ -240,7 +321,7 @@ __device__ __forceinline__ void store_values(const AppendArgs& a, int64_t r, int
 __device__ __forceinline__ bool breaks(int before, int slot) { return slot < 0 || before < 0 || (slot >> 4) != (before >> 4) || (slot & 15) == 0; }
 
 template <int L2>
-__global__ void __launch_bounds__(256) append_e4m3_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(256, L2 <= 8 ? 4 : 1) append_e4m3_kernel(AppendArgs a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if ((int64_t)blockIdx.x >= a.kv_grid) {        // queries: L2 lanes to a head, so many heads of a row to a wave that reads weights and angles once
     constexpr int HEADS = 64 / L2, PASSES = Q_PASSES;

@@ -95,6 +95,23 @@ def test_append_long_portion(T, before):
     _check_append(rows, q, pages, plain, None, step, ek, ev, eq)
 
 
+@pytest.mark.parametrize("Hkv,D", [(8, 128), (4, 256), (8, 80)])
+def test_append_keys_are_the_nearest_numbers(Hkv, D):
+    """Of 16 of the power on and up, where a number on the other side of a middle is off by two or more of the power. (In float32 alone one of
+    650,000 numbers is on the other side; below, cancellation may leave more than the 2^-20 within which numbers are done again.)"""
+    T, page, gen = 3000, 16, _gen(31)
+    step = Step([(T, 0), (T, 5000)], page, gen)
+    pages = empty_pages(step.pages, Hkv, D, page)
+    plain = PlainPages.of(pages)
+    rows, rows64 = _rows(step.T, 1, Hkv, D, gen)
+    w, table = torch.exp(0.3 * torch.randn(D, generator=gen)), rotation(8192, D)
+    ops.qk_norm_rope_store_e4m3(rows, w.to(DEV), w.to(DEV), EPS, table.to(DEV), step.positions.to(DEV), step.slots.to(DEV), pages, 1, Hkv, D, page)
+    _append_plain(rows64, step, plain, 1, Hkv, D, w, w, table)
+    got = PlainPages.of(pages)
+    large = plain.k.abs() >= 16
+    assert torch.equal(got.kp, plain.kp) and torch.equal(got.k[large], plain.k[large]) and int(large.sum()) > 0.5 * step.T * Hkv * D
+
+
 @pytest.mark.parametrize("norm,turn,same", [(False, True, False), (True, False, False), (False, False, False), (True, True, True), (False, False, True)])
 @pytest.mark.parametrize("offset", [0, 1])
 def test_append_options(norm, turn, same, offset):
