@@ -37,7 +37,7 @@ CORE_SOURCES = ["elementwise.hip", "rope_kv.hip", "attention_simple.hip",
                 "streams.hip", "kv_e4m3.hip"]
 ATTN_SOURCE = "attention_mfma.hip"
 ATTN_E4M3_SOURCE = "attention_e4m3.hip"
-HEADERS = ["common.h", "errors.inc", "sampling.h", "chunks.h", "e4m3.h"]
+HEADERS = ["common.h", "errors.inc", "sampling.h", "chunks.h", "e4m3.h", "kv_e4m3.h"]
 CALLS_SOURCE = "calls.cpp"
 # Head sizes that build_all() compiles ahead of use; any other multiple of 16 up to 512 is compiled when a model first needs it.
 DEFAULT_HEAD_DIMS = (16, 32, 48, 64, 80, 128, 256)

@@ -136,6 +136,7 @@ _ATTN_PROTOS = {
 }
 
 _ATTN_E4M3_PROTOS = {
+    "me_attn8_decode_fused": [P, L, P, L, P, P, F, P, L, P, P, P, P, L, P, I, I, P, I, I, I, I, F, I, I, I, I, P, P, I, P],
     "me_attn8_decode": [P, L, P, L, P, P, P, P, L, P, I, I, P, I, I, I, I, F, I, I, I, I, P, P, P],
     "me_attn8_prompt": [P, L, P, L, P, P, P, P, L, P, I, I, P, P, L, I, I, I, I, F, I, I, I, I, P, P, P],
 }
@@ -790,6 +791,50 @@ class HipBackend:
                      block_tables.data_ptr() + num_decodes * tables[0] * 4, *tables, context_lens.data_ptr() + num_decodes * 4,
                      prefill_cu.data_ptr(), Tp, B - num_decodes, Hq, Hkv, page, float(scale), int(window or 0), int(chunk or 0), part, parts,
                      _ptr(scratch), _ptr(sinks), stream)
+        return out
+
+    def decode_step_attention_e4m3(self, rows, q_weight, k_weight, eps, table, pages: PagesE4M3, page: int, block_tables, context_lens,
+                                   max_context: int, scale: float, window: int | None, Hq: int, Hkv: int, D: int, even_contexts: bool = False,
+                                   chunk: int | None = None, sinks=None, values_are_keys: bool = False) -> torch.Tensor:
+        """A pure decode step's `qk_norm_rope_store_e4m3` and `paged_attention_e4m3` as one launch, their results and bytes the same: rows
+        [B, (Hq+2Hkv)*D] as the packed product left them (values_are_keys: [B, (Hq+Hkv)*D]), row r request r's one new token at
+        position context_lens[r] - 1, whose key and value go to the page that the block table names for it (none, where it names none).
+        Up to 16 query heads to a key head. The rows stay as they were. Returns [B, Hq*D]."""
+        what = "decode_step_attention_e4m3"
+        if not (Hkv >= 1 and Hq >= 1 and Hq % Hkv == 0 and Hq // Hkv <= 16):
+            raise KernelError(f"{what}: {Hq} query heads over {Hkv} key heads; a key head takes up to 16, all alike")
+        if rows.dtype != torch.bfloat16:
+            raise KernelError(f"{what}: rows must be bfloat16, got {rows.dtype}")
+        B, width = rows.shape[0], (Hq + (1 if values_are_keys else 2) * Hkv) * D
+        if not (rows.dim() == 2 and rows.stride(1) == 1 and rows.shape[1] == width and (B <= 1 or rows.stride(0) >= width)):
+            raise KernelError(f"{what}: rows must be [B, {width}] with unit inner stride, got {tuple(rows.shape)}")
+        n = pages.check(what, Hkv, D, page)
+        for w in (q_weight, k_weight):
+            if not (w is None or (w.dtype == torch.float32 and w.shape == (D,) and w.is_contiguous())):
+                raise KernelError(f"{what}: norm weights must be float32 [D]")
+        if (q_weight is None) != (k_weight is None):
+            raise KernelError(f"{what}: give both norm weights or neither")
+        if not (table is None or (table.dtype == torch.float32 and table.is_contiguous() and table.dim() == 3 and table.shape[1:] == (D // 2, 2))):
+            raise KernelError(f"{what}: rotary table must be float32 [P, D/2, 2]")
+        if not (block_tables.dim() == 2 and block_tables.dtype == torch.int32 and block_tables.stride(1) == 1 and block_tables.shape[0] >= B
+                and block_tables.shape[1] >= 1 and _is_i32(context_lens, B)):
+            raise KernelError(f"{what}: block tables must be int32 [B, MB], contexts int32 [B]")
+        if (window and chunk) or (window or 0) < 0 or (chunk or 0) < 0:
+            raise KernelError(f"{what}: a window or a block, not both and neither of them negative")
+        if not (sinks is None or (sinks.dtype == torch.float32 and sinks.shape == (Hq,) and sinks.is_contiguous())):
+            raise KernelError(f"{what}: sinks must be float32 [Hq]")
+        stream = _check_device(what, rows, q_weight, k_weight, table, block_tables, context_lens, sinks, *pages.tensors())
+        out = torch.empty((B, Hq * D), dtype=rows.dtype, device=rows.device)
+        if B == 0:
+            return out
+        part, parts = decode_partitions_e4m3(B, Hq, Hkv, max_context, int(window or chunk or 0), even_contexts)
+        scratch = torch.empty(B * Hq * parts * (D + 2), dtype=torch.float32, device=rows.device) if parts > 1 else None
+        attn_e4m3_lib(D).call(
+            "me_attn8_decode_fused", rows.data_ptr(), max(rows.stride(0), width), out.data_ptr(), Hq * D, _ptr(q_weight), _ptr(k_weight), float(eps),
+            _ptr(table), 0 if table is None else table.shape[0], pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scales.data_ptr(),
+            pages.v_scales.data_ptr(), n, block_tables.data_ptr(), block_tables.stride(0) if block_tables.shape[0] > 1 else block_tables.shape[1],
+            block_tables.shape[1], context_lens.data_ptr(), B, Hq, Hkv, page, float(scale), int(window or 0), int(chunk or 0), part, parts,
+            _ptr(scratch), _ptr(sinks), int(bool(values_are_keys)), stream)
         return out
 
     # -- matrix products -----------------------------------------------------------------
@@ -2468,6 +2513,8 @@ def paged_attention(*a, **k): return backend().paged_attention(*a, **k)
 def decode_step_attention(*a, **k): return backend().decode_step_attention(*a, **k)
 def qk_norm_rope_store_e4m3(*a, **k): return backend().qk_norm_rope_store_e4m3(*a, **k)
 def paged_attention_e4m3(*a, **k): return backend().paged_attention_e4m3(*a, **k)
+def decode_step_attention_e4m3(*a, **k): return backend().decode_step_attention_e4m3(*a, **k)
+def decode_step_fuses_e4m3(Hq: int, Hkv: int) -> bool: return bool(FUSE_DECODE_STEP and hasattr(backend(), "decode_step_attention_e4m3") and Hq // Hkv <= 16)
 def linear(*a, **k): return backend().linear(*a, **k)
 def silu_mul_linear(*a, **k): return backend().silu_mul_linear(*a, **k)
 def norm_linear(*a, **k): return backend().norm_linear(*a, **k)

@@ -366,10 +366,17 @@ class Attention(Mixer):
         return self._project(o, packed)
 
     def _attend_e4m3(self, qkv, qw, kw, eps, table, step, cache, store):
-        """Norm, position, the write of this step's keys and values and attention, over pages of 8 bits."""
+        """Norm, position, the write of this step's keys and values and attention, over pages of 8 bits: in one launch where the step has
+        single tokens only."""
         Hq, Hkv, D = self.num_heads, self.num_kv_heads, self.head_dim
         grp = step.groups[cache.group]
         pages = ops.PagesE4M3(cache.k, cache.v, cache.tensors["k_scales"], cache.tensors["v_scales"])
+        if (store and step.num_decodes == step.num_tokens and (self.position is None or table is not None)
+                and ops.decode_step_fuses_e4m3(Hq, Hkv)):
+            return ops.decode_step_attention_e4m3(qkv, qw, kw, eps, table, pages, cache.page_size, grp.block_tables, step.context_lens,
+                                                  step.max_decode_context, self.scale, self.window, Hq, Hkv, D,
+                                                  even_contexts=step.decode_contexts_even, chunk=self.chunk, sinks=self.sinks,
+                                                  values_are_keys=self.values_are_keys)
         bound = max(step.max_decode_context, step.max_prefill_context)
         q = qkv[:, : self.q_size]
         if self.position is not None and table is None:

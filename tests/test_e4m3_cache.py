@@ -120,6 +120,31 @@ def test_attention_refusals():
     _refused(call, a, "no multiple", Hkv=3)
 
 
+def test_decode_step_refusals():
+    call = ops.HipBackend().decode_step_attention_e4m3
+    D, Hq, Hkv, page, B = 32, 4, 2, 16, 3
+    a = dict(rows=torch.zeros(B, (Hq + 2 * Hkv) * D, dtype=torch.bfloat16), q_weight=torch.ones(D), k_weight=torch.ones(D), eps=1e-6,
+             table=torch.zeros(8, D // 2, 2), pages=empty_pages(4, Hkv, D, page, "cpu"), page=page, block_tables=torch.zeros(B, 2, dtype=torch.int32),
+             context_lens=torch.zeros(B, dtype=torch.int32), max_context=4, scale=0.1, window=None, Hq=Hq, Hkv=Hkv, D=D)
+    _refused(call, a, "bfloat16", rows=a["rows"].float())
+    _refused(call, a, "rows must be", rows=a["rows"][:, :-1])
+    _refused(call, a, "rows must be", values_are_keys=True)
+    _refused(call, a, "query heads", Hkv=0)
+    _refused(call, a, "query heads", Hkv=3)
+    _refused(call, a, "query heads", Hq=34)
+    _refused(call, a, "both norm weights", k_weight=None)
+    _refused(call, a, "float32", q_weight=torch.ones(D, dtype=torch.bfloat16), k_weight=torch.ones(D, dtype=torch.bfloat16))
+    _refused(call, a, "rotary table", table=torch.zeros(8, D, 2))
+    _refused(call, a, "block tables", block_tables=a["block_tables"][:2])
+    _refused(call, a, "block tables", context_lens=a["context_lens"][:2])
+    _refused(call, a, "block tables", context_lens=a["context_lens"].long())
+    _refused(call, a, "window or a block", window=3, chunk=4)
+    _refused(call, a, "window or a block", window=-3)
+    _refused(call, a, "sinks", sinks=torch.zeros(3))
+    _refused(call, a, "power of two", page=24)
+    _refused(call, a, "current GPU" if torch.cuda.is_available() else "GPU")
+
+
 def test_libraries_of_other_head_sizes_are_refused():
     for D in (0, 8, 24, 272, 512):
         with pytest.raises(build.BuildError, match="multiple of 16"):

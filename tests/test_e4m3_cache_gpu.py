@@ -476,6 +476,89 @@ def test_captured_step_is_replayed():
             assert torch.equal(p.view(torch.uint8), o.view(torch.uint8))
 
 
+def _in_two(rows, pages, step, on, qw, kw, table, Hq, Hkv, D, page, scale, same, **options):
+    q = ops.qk_norm_rope_store_e4m3(rows, qw, kw, EPS, table, on["positions"], on["slots"], pages, Hq, Hkv, D, page, values_are_keys=same)
+    return ops.paged_attention_e4m3(q, pages, page, on["tables"], on["contexts"], on["seq"], on["positions"], None, step.decode, step.decode_context, scale,
+                                    options.get("window"), Hq, Hkv, D, chunk=options.get("chunk"), sinks=options.get("sinks"))
+
+
+def _copied(pages):
+    return ops.PagesE4M3(*(t.clone() for t in pages.tensors()))
+
+
+def _same_bytes(a, b):
+    return all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(a.tensors(), b.tensors()))
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", HEADS + [(32, 2, 64), (15, 1, 112)])
+@pytest.mark.parametrize("norm,turn,same,options", [(True, True, False, {}), (False, True, False, dict(window=100)), (True, False, True, dict(sinks=True)),
+                                                    (False, False, False, dict(chunk=48)), (True, True, True, dict(window=600, sinks=True))])
+def test_decode_step_in_one_launch(Hq, Hkv, D, norm, turn, same, options):
+    """The bits and the cache's bytes of the two launches: places of all kinds in a block, blocks that grow, one partition and many, a padding row."""
+    gen, page = _gen(D + norm), 32 if same else 16
+    step = Step([(1, k) for k in (0, 1, 14, 15, 16, 31, 63, 64, 65, -1, 300, 255, 700, 1029, 5000)], page, gen)
+    on = {n: getattr(step, n).to(DEV) for n in ("tables", "contexts", "seq", "positions", "slots")}
+    options = dict(options, sinks=torch.randn(Hq, generator=gen).to(DEV)) if options.get("sinks") else options
+    rows, _ = _rows(step.T, Hq, Hkv, D, gen, gap=8, values_are_keys=same)
+    qw, kw = ((1 + 0.2 * torch.randn(D, generator=gen)).to(DEV), torch.exp(torch.randn(D, generator=gen)).to(DEV)) if norm else (None, None)
+    table = rotation(8192, D).to(DEV) if turn else None
+    one = mild_pages(step.pages, Hkv, D, page, gen)
+    two, kept = _copied(one), rows.clone()
+    want = _in_two(rows, two, step, on, qw, kw, table, Hq, Hkv, D, page, D ** -0.5, same, **options)
+    got = ops.decode_step_attention_e4m3(rows, qw, kw, EPS, table, one, page, on["tables"], on["contexts"], step.decode_context, D ** -0.5,
+                                         options.get("window"), Hq, Hkv, D, chunk=options.get("chunk"), sinks=options.get("sinks"), values_are_keys=same)
+    assert _same_bytes(one, two) and torch.equal(got, want) and torch.equal(rows, kept) and not got[9].any()
+
+
+def test_decode_steps_one_after_another_in_a_graph():
+    """Tokens of several requests one by one across blocks and pages, the step replayed with what a step changes, against the two launches."""
+    Hq, Hkv, D, page, B = 8, 4, 128, 16, 5
+    gen = _gen(77)
+    tables = torch.randperm(B * 8, generator=gen).int().view(B, 8).to(DEV)
+    contexts = torch.tensor([1, 16, 40, 63, 64], dtype=torch.int32, device=DEV)
+    one = mild_pages(B * 8, Hkv, D, page, gen)
+    two, table, w = _copied(one), rotation(256, D).to(DEV), torch.ones(D, device=DEV)
+    rows = torch.zeros(B, (Hq + 2 * Hkv) * D, dtype=torch.bfloat16, device=DEV)
+
+    def run():
+        return ops.decode_step_attention_e4m3(rows, w, w, EPS, table, one, page, tables, contexts, 128, D ** -0.5, None, Hq, Hkv, D)
+    first = _copied(one)
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for x, y in zip(one.tensors(), first.tensors()):
+        x.view(torch.uint8).copy_(y.view(torch.uint8))
+    for i in range(40):
+        rows.copy_((1.1 ** i) * torch.randn(rows.shape, generator=gen))
+        graph.replay()
+        torch.cuda.synchronize()
+        at = contexts - 1
+        slots = tables.gather(1, (at // page).long()[:, None])[:, 0] * page + at % page
+        q = ops.qk_norm_rope_store_e4m3(rows, w, w, EPS, table, at, slots.int(), two, Hq, Hkv, D, page)
+        want = ops.paged_attention_e4m3(q, two, page, tables, contexts, torch.arange(B, dtype=torch.int32, device=DEV), at, None, B, 128, D ** -0.5, None, Hq, Hkv, D)
+        assert torch.equal(out, want) and _same_bytes(one, two)
+        contexts += 1
+
+
+def test_decode_step_without_a_page():
+    """A token whose table entry names no page is not written; it sees what the others hold, and nothing of itself."""
+    gen = _gen(5)
+    step = Step([(1, 40), (1, 16), (1, 0)], 16, gen)
+    pages, D = mild_pages(step.pages, 2, 64, 16, gen), 64
+    before = _copied(pages)
+    tables = step.tables.to(DEV)
+    for r, entry in ((0, -1), (1, 1 << 30), (2, -7)):
+        tables[r, int(step.contexts[r] - 1) // 16] = entry
+    rows = torch.randn(3, 8 * D, generator=gen).to(torch.bfloat16).to(DEV)
+    got = ops.decode_step_attention_e4m3(rows, None, None, EPS, None, pages, 16, tables, step.contexts.to(DEV), 41, 0.1, None, 4, 2, D)
+    assert _same_bytes(pages, before)
+    want = ops.paged_attention_e4m3(rows[:, :4 * D], pages, 16, tables, step.contexts.to(DEV), step.seq.to(DEV), step.positions.to(DEV), None, 3, 41, 0.1, None, 4, 2, D)
+    assert torch.equal(got, want) and not got[2].any()
+    assert ops.decode_step_attention_e4m3(rows[:0], None, None, EPS, None, pages, 16, tables, step.contexts.to(DEV), 41, 0.1, None, 4, 2, D).shape == (0, 4 * D)
+
+
 def test_calls_on_two_streams_do_not_meet():
     """Two launches side by side, both cut into partitions, on streams of their own."""
     gen = _gen(14)
