@@ -165,7 +165,8 @@ __device__ __forceinline__ int row_slot(const AppendArgs& a, int64_t t) {
 // Whether a number, scaled for its block, lies so near to the middle between two e4m3 numbers that float32 may have put it on the other side:
 // within 8 of its steps. There it would be off by a whole step of e4m3 (one number in 650,000 was, most of them by one of the large
 // steps; what cancellation leaves further off is small, and so are its steps); one in 65,000 is done again by norm_rotate_key. 60 rows
-// of one token 6.4 us in float32 alone, 8.4 so; 7,900 rows of 32 and 8 heads of 128 48.5 and 51, with every key done so 59, all in double 66.
+// of one token 6.4 us in float32 alone, 8.4 so; 7,900 rows of 32 and 8 heads of 128 48.5 and 49.6 (53 where the queries' waves have 132
+// registers instead of 128), with every key done so 59, all in double 66.
 __device__ __forceinline__ bool between(float x) { return ((__float_as_uint(x) + 0x80008u) & 0xfffffu) < 0x10u; }
 
 // The cnt rows from r on, of one block, of one key head (at most 16, ascending slots). Lane i holds the slot and the position of row r + i
@@ -213,6 +214,14 @@ __device__ __forceinline__ void store_keys(const AppendArgs& a, int64_t r, int c
     for (int j = lane; j < begin * a.D / 4; j += 64) held[j] = e4_again(held[j], back);
   }
   const float scale = e4_pow2(-power);
+  auto place = [&](int p, float (&y1)[8], float (&y2)[8]) {
+    const int at_block = __shfl(slots, row_of(p)) & (E4_BLOCK - 1);
+    if (!active || p * TOKENS + lane / L2 >= cnt) return;
+    uint8_t* dst = base + (int64_t)at_block * a.D + 8 * l;
+    *reinterpret_cast<u32x2*>(dst) = u32x2{e4_pack(y1[0], y1[1], y1[2], y1[3]), e4_pack(y1[4], y1[5], y1[6], y1[7])};
+    *reinterpret_cast<u32x2*>(dst + half) = u32x2{e4_pack(y2[0], y2[1], y2[2], y2[3]), e4_pack(y2[4], y2[5], y2[6], y2[7])};
+  };
+  int again = 0;
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
     if (p > 0 && p * TOKENS >= cnt) continue;
@@ -222,22 +231,25 @@ __device__ __forceinline__ void store_keys(const AppendArgs& a, int64_t r, int c
       x1[p][j] = e4_scaled(x1[p][j], scale); x2[p][j] = e4_scaled(x2[p][j], scale);
       near |= between(x1[p][j]) | between(x2[p][j]);
     }
-    if (__builtin_expect(__any(near), 0)) {        // everything once more, asked for again (held until here, it would cost the queries' waves their registers)
-      asm volatile("" ::: "memory");
-      bf16x8 again1, again2;
-      Turn t;
-      Weights again;
-      load(p, again1, again2, t);
-      load_weights(a, a.k_w, at, again);
-      norm_rotate_key<L2>(a, a.k_w != nullptr, again, t, again1, again2, active, x1[p], x2[p]);
+    place(p, x1[p], x2[p]);
+    if (__any(near)) again |= 1 << p;
+  }
+  // Once more where it matters, everything asked for again and written over what has been: nothing is held for it, which would cost the waves
+  // of queries their registers.
+#pragma unroll 1
+  for (int p = 0; __builtin_expect(again >> p, 0); ++p) {
+    if (!(again >> p & 1)) continue;
+    asm volatile("" ::: "memory");
+    bf16x8 t1, t2;
+    Turn t;
+    Weights weights;
+    load(p, t1, t2, t);
+    load_weights(a, a.k_w, at, weights);
+    float y1[8], y2[8];
+    norm_rotate_key<L2>(a, a.k_w != nullptr, weights, t, t1, t2, active, y1, y2);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) { x1[p][j] = e4_scaled(x1[p][j], scale); x2[p][j] = e4_scaled(x2[p][j], scale); }
-    }
-    const int place = __shfl(slots, row_of(p)) & (E4_BLOCK - 1);
-    if (!active || p * TOKENS + lane / L2 >= cnt) continue;
-    uint8_t* dst = base + (int64_t)place * a.D + 8 * l;
-    *reinterpret_cast<u32x2*>(dst) = u32x2{e4_pack(x1[p][0], x1[p][1], x1[p][2], x1[p][3]), e4_pack(x1[p][4], x1[p][5], x1[p][6], x1[p][7])};
-    *reinterpret_cast<u32x2*>(dst + half) = u32x2{e4_pack(x2[p][0], x2[p][1], x2[p][2], x2[p][3]), e4_pack(x2[p][4], x2[p][5], x2[p][6], x2[p][7])};
+    for (int j = 0; j < 8; ++j) { y1[j] = e4_scaled(y1[j], scale); y2[j] = e4_scaled(y2[j], scale); }
+    place(p, y1, y2);
   }
   if (lane == 0) *code = (uint8_t)(power + E4_BIAS);
 }
