@@ -2476,6 +2476,12 @@ def decode_step_fuses(dtype: torch.dtype, D: int, page: int) -> bool:
                 and page & (page - 1) == 0)
 
 
+def decode_step_fuses_e4m3(rows: torch.Tensor, Hq: int, Hkv: int) -> bool:
+    """Whether `decode_step_attention_e4m3` takes these rows: 16 query heads to a key head at most, rows that begin at multiples of 16 bytes."""
+    return bool(FUSE_DECODE_STEP and hasattr(backend(), "decode_step_attention_e4m3") and Hq // Hkv <= 16 and rows.stride(0) % 8 == 0
+                and rows.data_ptr() % 16 == 0)
+
+
 def decode_contexts_even(num_seqs: int, min_context: int, max_context: int) -> bool:
     """Whether the decode kernel may keep each request's work on one XCD (8 requests or more whose
     contexts differ by 5 % at most), or has to spread every request over the XCDs. With all of a request
@@ -2514,7 +2520,6 @@ def decode_step_attention(*a, **k): return backend().decode_step_attention(*a, *
 def qk_norm_rope_store_e4m3(*a, **k): return backend().qk_norm_rope_store_e4m3(*a, **k)
 def paged_attention_e4m3(*a, **k): return backend().paged_attention_e4m3(*a, **k)
 def decode_step_attention_e4m3(*a, **k): return backend().decode_step_attention_e4m3(*a, **k)
-def decode_step_fuses_e4m3(Hq: int, Hkv: int) -> bool: return bool(FUSE_DECODE_STEP and hasattr(backend(), "decode_step_attention_e4m3") and Hq // Hkv <= 16)
 def linear(*a, **k): return backend().linear(*a, **k)
 def silu_mul_linear(*a, **k): return backend().silu_mul_linear(*a, **k)
 def norm_linear(*a, **k): return backend().norm_linear(*a, **k)

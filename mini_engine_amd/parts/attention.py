@@ -372,7 +372,7 @@ class Attention(Mixer):
         grp = step.groups[cache.group]
         pages = ops.PagesE4M3(cache.k, cache.v, cache.tensors["k_scales"], cache.tensors["v_scales"])
         if (store and step.num_decodes == step.num_tokens and (self.position is None or table is not None)
-                and ops.decode_step_fuses_e4m3(Hq, Hkv)):
+                and ops.decode_step_fuses_e4m3(qkv, Hq, Hkv)):
             return ops.decode_step_attention_e4m3(qkv, qw, kw, eps, table, pages, cache.page_size, grp.block_tables, step.context_lens,
                                                   step.max_decode_context, self.scale, self.window, Hq, Hkv, D,
                                                   even_contexts=step.decode_contexts_even, chunk=self.chunk, sinks=self.sinks,

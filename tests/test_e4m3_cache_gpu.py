@@ -510,6 +510,22 @@ def test_decode_step_in_one_launch(Hq, Hkv, D, norm, turn, same, options):
     assert _same_bytes(one, two) and torch.equal(got, want) and torch.equal(rows, kept) and not got[9].any()
 
 
+def test_decode_step_rows_that_do_not_fit():
+    """Rows off the steps of 16 bytes go to the two launches, which take them, and so do more than 16 query heads to a key head."""
+    gen = _gen(3)
+    step = Step([(1, 40), (1, 16)], 16, gen)
+    pages = mild_pages(step.pages, 2, 32, 16, gen)
+    args = (None, None, EPS, None, pages, 16, step.tables.to(DEV), step.contexts.to(DEV), 41, 0.1, None)
+    for gap, offset, fits in ((0, 0, True), (8, 8, True), (4, 0, False), (8, 4, False)):
+        rows, _ = _rows(2, 4, 2, 32, gen, gap=gap, offset=offset)
+        assert ops.decode_step_fuses_e4m3(rows, 4, 2) == fits
+        if not fits:
+            with pytest.raises(ops.KernelError, match="aligned|alignment"):
+                ops.decode_step_attention_e4m3(rows, *args, 4, 2, 32)
+    rows, _ = _rows(2, 34, 2, 32, gen)
+    assert not ops.decode_step_fuses_e4m3(rows, 34, 2)
+
+
 def test_decode_steps_one_after_another_in_a_graph():
     """Tokens of several requests one by one across blocks and pages, the step replayed with what a step changes, against the two launches."""
     Hq, Hkv, D, page, B = 8, 4, 128, 16, 5
