@@ -43,7 +43,7 @@ CALLS_SOURCE = "calls.cpp"
 DEFAULT_HEAD_DIMS = (16, 32, 48, 64, 80, 128, 256)
 CAPPED_HEAD_DIMS = (32, 64, 128)          # ... of the variant with a cap on the scores
 DISTANCE_HEAD_DIMS = (16, 32, 48, 64, 128)          # ... of the variant with slopes times distances
-E4M3_HEAD_DIMS = (16, 32, 48, 64, 80, 128, 256)          # ... of the attention over an 8-bit cache
+E4M3_HEAD_DIMS = (16, 32, 48, 64, 80, 96, 112, 128, 144, 256)          # ... of the attention over an 8-bit cache
 
 _locks: dict = {}
 _locks_guard = threading.Lock()
