@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attn8_decode_kernel(At
   for (int dt = 0; dt < DT; ++dt) c.acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   bf16_t* queries = reinterpret_cast<bf16_t*>(lds + ((4 * ncols * (HD + 2) + 3) & ~3));
   if constexpr (FUSED) {
-    const int position = w.table ? min(max(pos, 0), w.table_positions - 1) : 0;
+    const int position = w.table ? min(max(pos, 0), w.table_positions - 1) : 0;      // (beyond the table only past the host's largest context)
     constexpr int HEADS = 64 / HEAD_LANES;
     for (int i = wave * HEADS + lane / HEAD_LANES; i - lane / HEAD_LANES < ncols; i += 4 * HEADS) {
       const int l = lane % HEAD_LANES;

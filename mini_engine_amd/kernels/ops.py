@@ -816,6 +816,8 @@ class HipBackend:
             raise KernelError(f"{what}: give both norm weights or neither")
         if not (table is None or (table.dtype == torch.float32 and table.is_contiguous() and table.dim() == 3 and table.shape[1:] == (D // 2, 2))):
             raise KernelError(f"{what}: rotary table must be float32 [P, D/2, 2]")
+        if table is not None and max_context > table.shape[0]:
+            raise KernelError(f"{what}: a context of {max_context} tokens is beyond the rotation table's {table.shape[0]} positions")
         if not (block_tables.dim() == 2 and block_tables.dtype == torch.int32 and block_tables.stride(1) == 1 and block_tables.shape[0] >= B
                 and block_tables.shape[1] >= 1 and _is_i32(context_lens, B)):
             raise KernelError(f"{what}: block tables must be int32 [B, MB], contexts int32 [B]")

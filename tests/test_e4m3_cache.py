@@ -135,6 +135,7 @@ def test_decode_step_refusals():
     _refused(call, a, "both norm weights", k_weight=None)
     _refused(call, a, "float32", q_weight=torch.ones(D, dtype=torch.bfloat16), k_weight=torch.ones(D, dtype=torch.bfloat16))
     _refused(call, a, "rotary table", table=torch.zeros(8, D, 2))
+    _refused(call, a, "beyond the rotation table", max_context=9)
     _refused(call, a, "block tables", block_tables=a["block_tables"][:2])
     _refused(call, a, "block tables", context_lens=a["context_lens"][:2])
     _refused(call, a, "block tables", context_lens=a["context_lens"].long())
