@@ -1693,14 +1693,15 @@ def _scratch(num_floats: int, device, use: str = "decode") -> torch.Tensor:
 
 
 def decode_partitions_e4m3(num_seqs: int, Hq: int, Hkv: int, max_context: int, span: int = 0, even: bool = False) -> tuple:
-    """(keys per partition, partitions) of a launch of single tokens over an 8-bit cache. Up to 512 keys in one piece, a launch and a
-    join saved (one row of 489 keys, 16 heads over 8: 6.5 us, in two pieces 8.5); longer ranges in steps of 256 keys into as many
+    """(keys per partition, partitions) of a launch of single tokens over an 8-bit cache. Up to 640 keys (a window of
+    512 whatever its place) in one piece, a launch and a join saved (one row of 489 keys, 16 heads over 8: 6.5 us, in two pieces 8.5; 23 of
+    575, 32 heads over 8, 11.9 and 13.7; 8 of 640 9.9 and 9.1); longer ranges in steps of 256 keys into as many
     pieces as give 512 workgroups, two for each CU: one row of 8,192 keys, 32 heads over 8, 11.8 us in pieces of 256 (1,024: 18.6; whole
     51), 8 of 8,192 30.2 in pieces of 1,024 (256: 36.9, 4,096: 57), 64 of 2,048 49.6 whole (512: 55.6). 1,536 workgroups where
     requests are not equally long, for the short ones leave early: 61 of up to 4,096 61.7 us in pieces of 1,024, 72 of 2,048."""
     keys = max(1, min(max_context, span + 63) if span else max_context)
-    if keys <= 512:
-        return 512, 1
+    if keys <= 640:
+        return 640, 1
     base = num_seqs * Hkv * -(-(Hq // Hkv) // 16)
     parts = min(-(-(512 if even or num_seqs == 1 else 1536) // base), -(-keys // 256))
     part = -(-keys // (parts * 256)) * 256
