@@ -380,8 +380,10 @@ class PagesE4M3:
 
     def check(self, what: str, Hkv: int, D: int, page: int) -> int:
         """Raises unless the tensors are such pages; returns how many there are."""
-        _check(page >= self.BLOCK and page & (page - 1) == 0, f"{what}: a page has a power of two of tokens, 16 or more, not {page}")
-        _check(D % 16 == 0 and 16 <= D <= 256, f"{what}: the head size must be a multiple of 16 up to 256, not {D}")
+        if page < self.BLOCK or page & (page - 1):
+            raise KernelError(f"{what}: a page has a power of two of tokens, 16 or more, not {page}")
+        if D % 16 or not 16 <= D <= 256:
+            raise KernelError(f"{what}: the head size must be a multiple of 16 up to 256, not {D}")
         k, v = self.k, self.v
         shape = k.shape
         n = shape[0] if shape else 0
@@ -728,7 +730,7 @@ class HipBackend:
         if not (_is_i32(positions, T) and _is_i32(slots, T)):
             raise KernelError(f"{what}: positions and slots must be int32 [T]")
         stream = _check_device(what, rows, q_weight, k_weight, table, positions, slots, *pages.tensors())
-        q = torch.empty((T, Hq * D), dtype=rows.dtype, device=rows.device)
+        q = rows.new_empty(T, Hq * D)
         core().call("me_append_e4m3", rows.data_ptr(), max(rows.stride(0), width), q.data_ptr(), _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(table),
                     0 if table is None else table.shape[0], int(position_bound), positions.data_ptr(), slots.data_ptr(), pages.k.data_ptr(),
                     pages.v.data_ptr(), pages.k_scales.data_ptr(), pages.v_scales.data_ptr(), n, T, Hq, Hkv, D, page,
@@ -769,7 +771,7 @@ class HipBackend:
         if not (T == num_decodes or (B > num_decodes and prefill_cu is not None and _is_i32(prefill_cu, B - num_decodes + 1))):
             raise KernelError(f"{what}: prefill_cu must be int32 [B-Dn+1]")
         stream = _check_device(what, q, block_tables, context_lens, prefill_cu, sinks, *pages.tensors())
-        out = torch.empty((T, Hq * D), dtype=q.dtype, device=q.device)
+        out = q.new_empty(T, Hq * D)
         if T == 0:
             return out
         lib, span = attn_e4m3_lib(D), int(window or chunk or 0)      # no query sees more keys than `span` (0: all of them)
@@ -826,7 +828,7 @@ class HipBackend:
         if not (sinks is None or (sinks.dtype == torch.float32 and sinks.shape == (Hq,) and sinks.is_contiguous())):
             raise KernelError(f"{what}: sinks must be float32 [Hq]")
         stream = _check_device(what, rows, q_weight, k_weight, table, block_tables, context_lens, sinks, *pages.tensors())
-        out = torch.empty((B, Hq * D), dtype=rows.dtype, device=rows.device)
+        out = rows.new_empty(B, Hq * D)
         if B == 0:
             return out
         part, parts = decode_partitions_e4m3(B, Hq, Hkv, max_context, int(window or chunk or 0), even_contexts)
