@@ -763,9 +763,15 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
         if (i == 12) { __builtin_amdgcn_sched_barrier(0); read_values(DC, 2 * DC); }
 #pragma unroll
         for (int j = 0; j < CB; ++j)
-          if (i == 16 * j / CB) { sn = score(j, j ? sn : zero); asm volatile("" : "+v"(sn)); __builtin_amdgcn_sched_barrier(0); }
+          if (i == 16 * j / CB) {
+            sn = score(j, j ? sn : zero);
+            // (beyond 128 channels every product's sums would be moved between registers for it: 300 tokens over 2,800 keys 111 us for 85)
+            if constexpr (HD <= 128) asm volatile("" : "+v"(sn));
+            __builtin_amdgcn_sched_barrier(0);
+          }
         pb[i >> 3][i & 7] = static_cast<bf16_t>(weigh(i));
       }
+      asm volatile("" : "+v"(sn));            // (wanted in the next step only: the products would be moved behind everything that follows)
       float sum = sum_up();
       // The reference point is raised only when a weight got large, and the block's weights are taken again.
       if (__builtin_expect(__any(sum > MOST_WEIGHT), 0)) {

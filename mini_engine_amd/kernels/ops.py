@@ -1715,13 +1715,15 @@ def prompt_partitions_e4m3(tokens: int, num_seqs: int, Hq: int, Hkv: int, D: int
 
     A workgroup walks a range at 17 ns a key while most of them have a compute unit to themselves (up to 128), 22 ns up to 256, 27 ns two
     to a unit, and in turns beyond 512; partial results of partitions are written and read at 4 TB/s, and joining them is a launch
-    of 5 us. The number of partitions that this makes cheapest, of at least 256 keys. 32 heads over 8 of 128: 489 tokens over
-    8,192 keys 135 us whole, 92 in 3, 82 in 4, 91 in 8; 256 over 32,256 keys 553 whole, 203 in 4, 138 in 8; 2,000 over 8,000 keys 222
-    whole, 247 in 2; 16 over 8: 2,048 tokens from the start 44 whole, 56 in 2."""
+    of 5 us. At other head sizes than 128 a walk takes three quarters and a 512th of the head size of that, beyond 128 (one workgroup to
+    a unit) a 95th of the head size. The number of partitions that this makes cheapest, of at least 256 keys. 32 heads over 8 of 128:
+    489 tokens over 8,192 keys 135 us whole, 92 in 3, 80 in 4, 91 in 8; 256 over 32,256 keys 500 whole, 200 in 4, 134 in 8; 2,000 over
+    8,000 keys 212 whole, 240 in 2; 16 over 8: 2,048 tokens from the start 44 whole, 56 in 2; 6 over 2 of 32: 1,500 from the start 28
+    whole, 19 in 4; 16 over 2 of 256: the same 81 whole, 68 in 2."""
     G = Hq // Hkv
     keys = max(1, min(max_context, span + 128 // G + 64) if span else max_context)
     tiles = max(1, tokens * G // 128) * Hkv
-    most, size = keys // 256, D / 128
+    most, size = keys // 256, 0.75 + D / 512 if D <= 128 else D / 95
     best, parts = None, 1
     for p in (1, 128 // tiles, 256 // tiles, 512 // tiles, 1024 // tiles) if tiles <= 512 and most > 1 else ():
         p = max(1, min(p, most))
