@@ -563,10 +563,13 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
     uint32_t codes = ask_codes(seg_lo, more_pages), more_codes = 0;
     // bits 2 k and 2 k + 1: block k's groups lie in pages; of the last 32 blocks looked up and of the 32 before
     uint64_t held = __ballot(more_pages >= 0), held_before = 0;
-    // the first block from tile_from on that does not wholly lie in pages, as far as is known
-    const int first_whole = max(tile_from - seg_lo + PB - 1, 0) / PB;
+    // first_steady, first_whole: the first block that the wave, that every column of the tile sees whole; steady steps begin where their own
+    // block is the wave's and the one two on, whose values they convert, the tile's. clear: the first block from there on that does not wholly
+    // lie in pages, as far as is known.
+    const int first_steady = max(all_lo - seg_lo + PB - 1, 0) / PB, first_whole = max(tile_from - seg_lo + PB - 1, 0) / PB;
+    const int begin_steady = max(first_steady, first_whole - 2);
     auto clear_upto = [&](int k0) {
-      const int skip = first_whole - k0;
+      const int skip = begin_steady - k0;
       const uint64_t missing = skip >= 32 ? 0 : ~held & (~0ull << (2 * max(skip, 0)));
       return k0 + (missing ? __builtin_ctzll(missing) / 2 : 32);
     };
@@ -837,10 +840,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
     };
     // Blocks are walked in ascending order: in front of the window's first whole block, those that the wave sees whole (steady as long as every
     // group has its page), the rest. Loops of their own: where the ways through a step meet, the sums would change their registers.
-    const int first_steady = max(all_lo - seg_lo + PB - 1, 0) / PB;
     const int end_steady = __builtin_amdgcn_readfirstlane(all_hi >= seg_lo && tile_upto >= seg_lo ? min(min((all_hi + 1 - seg_lo) / PB, (tile_upto + 1 - seg_lo) / PB - 2), nblk) : 0);
     int k = 0;
-    for (; k < min(max(first_steady, first_whole - 2), nblk); ++k) { step(std::false_type{}, k, scores, scores_next); scores = scores_next; }
+    for (; k < min(begin_steady, nblk); ++k) { step(std::false_type{}, k, scores, scores_next); scores = scores_next; }
     for (; k + 1 < min(end_steady, clear - 2); k += 2) { step(std::true_type{}, k, scores, scores_next); step(std::true_type{}, k + 1, scores_next, scores); }
     for (; k < nblk; ++k) { step(std::false_type{}, k, scores, scores_next); scores = scores_next; }
     brought<0>();                             // (what was asked for beyond the last block lands before the LDS is another workgroup's)

@@ -399,6 +399,29 @@ def test_attention_tables_with_holes():
     assert ((got - o).abs() <= attention_bound(o, spread)).all() and not got[1].any()
 
 
+@pytest.mark.parametrize("Hq,Hkv,D", [(2, 2, 64), (4, 2, 128), (3, 3, 256)])
+@pytest.mark.parametrize("hole", [900, 970, 1000, 1030, 1060, 1300])
+def test_attention_windows_with_holes(Hq, Hkv, D, hole):
+    """A block without a page inside the windows of a tile's first tokens and in front of its last ones', and further on: none of its keys is seen,
+    whatever page 0, whose bytes are read in their place, holds."""
+    gen, page = _gen(D + hole), 32
+    step = Step([(140, 1500)], page, gen)
+    pages = mild_pages(step.pages, Hkv, D, page, gen)
+    spare = next(p for p in range(step.pages) if p not in step.table_rows[0])
+    step.table_rows[0] = [spare if p == 0 else p for p in step.table_rows[0]]
+    step.table_rows[0][hole // page] = -1
+    step.tables = torch.tensor(step.table_rows, dtype=torch.int32)
+    pages.k.view(torch.uint8)[0] = 0x7F
+    pages.v.view(torch.uint8)[0] = 0x7F
+    q = torch.randn(step.T, Hq * D, generator=gen).to(torch.bfloat16)
+    got = _attention(q.to(DEV), pages, step, D ** -0.5, Hq, Hkv, D, window=600).cpu().double().view(step.T, Hq, D)
+    numbers = PlainPages.of(pages).numbers()
+    for x in numbers:
+        x[0] = 0.0            # (the plain form takes its hidden keys from page 0 too, and drops them)
+    o, spread = attend(q.double().view(step.T, Hq, D), numbers, step, D ** -0.5, Hq, Hkv, window=600)
+    assert ((got - o).abs() <= attention_bound(o, spread)).all()
+
+
 def test_attention_of_no_rows():
     pages = mild_pages(2, 2, 32, 16, _gen(0))
     z = torch.zeros(0, dtype=torch.int32, device=DEV)
