@@ -601,7 +601,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) raw_v[i] = *reinterpret_cast<const u32x4v*>(lds_bytes + AT_RAW + (k & 3) * RAW + mine + 1024 * i);
     };
-    // Half j of block k's values. Keys in front of tile_lo, or from L on, or in no page become zeros; a NaN among the others is reported.
+    // Half j of block k's values. Keys in front of tile_lo, or from seg_hi on (up to two blocks more are turned than walked), or in no page
+    // become zeros; a NaN among the others is reported: one that some column of the tile sees.
     // WHOLE: every column of the tile sees all of the block, and it lies in pages.
     auto store_values = [&](auto whole_tag, int j, int k, uint32_t code, uint32_t there, char* vbuf) {
       constexpr bool WHOLE = decltype(whole_tag)::value;
@@ -612,8 +613,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 
         uint32_t w0 = raw_v[i][2 * j], w1 = raw_v[i][2 * j + 1];
         if constexpr (!WHOLE) {
           const int first = seg_lo + PB * k + 16 * group;
-          if (!((there >> group) & 1) || first < tile_lo || first + 16 > L) {
-            const int from = ((there >> group) & 1) ? tile_lo - first - 8 * j : 8, to = L - first - 8 * j;
+          if (!((there >> group) & 1) || first < tile_lo || first + 16 > seg_hi) {
+            const int from = ((there >> group) & 1) ? tile_lo - first - 8 * j : 8, to = seg_hi - first - 8 * j;
             const uint64_t upto = to >= 8 ? ~0ull : to <= 0 ? 0ull : (1ull << (8 * to)) - 1, below = from >= 8 ? ~0ull : from <= 0 ? 0ull : (1ull << (8 * from)) - 1;
             const uint64_t keep = upto & ~below;
             w0 &= (uint32_t)keep; w1 &= (uint32_t)(keep >> 32);

@@ -345,6 +345,25 @@ def test_attention_nan_in_a_value(D):
         assert int(torch.isnan(got).sum()) == seen * 2 and torch.isnan(got[:, 2:, 7]).sum() == seen * 2
 
 
+@pytest.mark.parametrize("Hq,Hkv,D", [(2, 2, 64), (4, 2, 128), (3, 3, 256), (6, 2, 48)])
+@pytest.mark.parametrize("new,before,window", [(300, 0, None), (300, 5, 100), (200, 1000, None)])
+def test_attention_nan_in_a_later_value(Hq, Hkv, D, new, before, window):
+    """A value that is NaN behind a tile's last token changes no bit of the tile's rows, not by another way of computing them either: the walk
+    reads up to two blocks further than the rows see."""
+    gen, page = _gen(D), 16
+    step = Step([(new, before)], page, gen)
+    pages = mild_pages(step.pages, Hkv, D, page, gen)
+    q = torch.randn(step.T, Hq * D, generator=gen).to(torch.bfloat16).to(DEV)
+    clean = _attention(q, pages, step, D ** -0.5, Hq, Hkv, D, window=window)
+    tile = 128 // (Hq // Hkv)                 # tokens that lie wholly in the first tile; one more may lie there in part
+    for at in (before + -(-128 // (Hq // Hkv)), before + tile + 41):
+        one = _copied(pages)
+        one.v.view(torch.uint8)[step.table_rows[0][at // page], :, 3, at % page] = 0x7F
+        got = _attention(q, one, step, D ** -0.5, Hq, Hkv, D, window=window)
+        assert torch.equal(got[:tile], clean[:tile])
+        assert torch.isnan(got[at - before].view(Hq, D)[:, 3]).all() and int(torch.isnan(got[at - before]).sum()) == Hq
+
+
 def test_attention_nan_where_nobody_looks():
     """Foreign and unwritten places hold NaN, in pages of others, behind the context and in front of the window: no row may notice. A key or a
     value that is NaN makes NaN of the rows (the value: of its channel in the rows) that see it, and of no other."""
