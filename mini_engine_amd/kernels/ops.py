@@ -779,7 +779,7 @@ class HipBackend:
         pools = (pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scales.data_ptr(), pages.v_scales.data_ptr(), n)
         tables = (block_tables.stride(0) if block_tables.shape[0] > 1 else block_tables.shape[1], block_tables.shape[1])
         if num_decodes > 0:
-            part, parts = decode_partitions_e4m3(num_decodes, Hq, Hkv, max_decode_context, span, even_contexts)
+            part, parts = decode_partitions_e4m3(num_decodes, Hq, Hkv, max_decode_context, span, even_contexts, D)
             # (from torch's allocator, which knows the stream and a capture's memory: calls on two streams never share it)
             scratch = torch.empty(num_decodes * Hq * parts * (D + 2), dtype=torch.float32, device=q.device) if parts > 1 else None
             lib.call("me_attn8_decode", q.data_ptr(), rows, out.data_ptr(), Hq * D, *pools, block_tables.data_ptr(), *tables,
@@ -831,7 +831,7 @@ class HipBackend:
         out = rows.new_empty(B, Hq * D)
         if B == 0:
             return out
-        part, parts = decode_partitions_e4m3(B, Hq, Hkv, max_context, int(window or chunk or 0), even_contexts)
+        part, parts = decode_partitions_e4m3(B, Hq, Hkv, max_context, int(window or chunk or 0), even_contexts, D)
         scratch = torch.empty(B * Hq * parts * (D + 2), dtype=torch.float32, device=rows.device) if parts > 1 else None
         attn_e4m3_lib(D).call(
             "me_attn8_decode_fused", rows.data_ptr(), max(rows.stride(0), width), out.data_ptr(), Hq * D, _ptr(q_weight), _ptr(k_weight), float(eps),
@@ -1694,17 +1694,21 @@ def _scratch(num_floats: int, device, use: str = "decode") -> torch.Tensor:
     return buf
 
 
-def decode_partitions_e4m3(num_seqs: int, Hq: int, Hkv: int, max_context: int, span: int = 0, even: bool = False) -> tuple:
-    """(keys per partition, partitions) of a launch of single tokens over an 8-bit cache. Up to 640 keys (a window of
-    512 whatever its place) in one piece, a launch and a join saved (one row of 489 keys, 16 heads over 8: 6.5 us, in two pieces 8.5; 23 of
-    575, 32 heads over 8, 11.9 and 13.7; 8 of 640 9.9 and 9.1); longer ranges in steps of 256 keys into as many
-    pieces as give 512 workgroups, two for each CU: one row of 8,192 keys, 32 heads over 8, 11.8 us in pieces of 256 (1,024: 18.6; whole
-    51), 8 of 8,192 30.2 in pieces of 1,024 (256: 36.9, 4,096: 57), 64 of 2,048 49.6 whole (512: 55.6). 1,536 workgroups where
-    requests are not equally long, for the short ones leave early: 61 of up to 4,096 61.7 us in pieces of 1,024, 72 of 2,048."""
+def decode_partitions_e4m3(num_seqs: int, Hq: int, Hkv: int, max_context: int, span: int = 0, even: bool = False, D: int = 128) -> tuple:
+    """(keys per partition, partitions) of a launch of single tokens over an 8-bit cache. Up to 512 keys in one piece, a launch and a
+    join saved (one row of 500 keys, 16 heads over 8 of 128: 6.4 us, in two pieces 7.5). Up to 640 (a window of 512 whatever its place) in
+    pieces of 256 only where a walk takes more than a join, which is beyond heads of 96, and where all pieces have a place at once, two
+    workgroups to a CU, one beyond heads of 128. Whole and in pieces, 575 keys: 16 heads over 8 of 128: one row 7.4 and 7.5, 8 rows 10.3
+    and 9.1, 16 10.8 and 10.0, 23 11.2 and 13.4, 64 17.3 and 17.1; 16 over 2 of 256: one 15.3 and 12.2, 32 19.0 and 15.2, 64 19.8 and
+    23.5; 16 over 8 of 96: 8 rows 8.7 and 8.2, 16 9.1 and 9.5; 32 over 8 of 64: one 5.2 and 6.2, 23 7.5 and 8.8. Longer ranges go in
+    steps of 256 keys into as many pieces as give 512 workgroups, two for each CU: one row of 8,192 keys, 32 heads over 8, 11.8 us in
+    pieces of 256 (1,024: 18.6; whole 51), 8 of 8,192 30.2 in pieces of 1,024 (256: 36.9, 4,096: 57), 64 of 2,048 49.6 whole (512: 55.6).
+    1,536 workgroups where requests are not equally long, for the short ones leave early: 61 of up to 4,096 61.7 us in pieces of 1,024, 72
+    of 2,048."""
     keys = max(1, min(max_context, span + 63) if span else max_context)
-    if keys <= 640:
-        return 640, 1
     base = num_seqs * Hkv * -(-(Hq // Hkv) // 16)
+    if keys <= 512 or keys <= 640 and (D <= 96 or base * -(-keys // 256) > (512 if D <= 128 else 256)):
+        return 640, 1
     parts = min(-(-(512 if even or num_seqs == 1 else 1536) // base), -(-keys // 256))
     part = -(-keys // (parts * 256)) * 256
     return part, -(-keys // part)

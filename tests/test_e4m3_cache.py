@@ -177,6 +177,16 @@ def test_partitions_cover_the_keys(B, Hq, Hkv, ctx, span):
             assert part % 64 == 0 and part > 0 and part * parts >= (min(ctx, span + rows + 62) if span else ctx)
 
 
+@pytest.mark.parametrize("B,Hq,Hkv,D,ctx,span,pieces", [
+    (8, 16, 8, 128, 640, 0, 3), (8, 16, 8, 128, 513, 0, 3), (16, 32, 8, 128, 1700, 512, 3), (8, 16, 8, 128, 512, 0, 1), (23, 32, 8, 128, 1700, 512, 1),
+    (64, 16, 8, 128, 640, 0, 1), (1, 16, 2, 256, 575, 0, 3), (32, 16, 2, 256, 575, 0, 3), (64, 16, 2, 256, 575, 0, 1), (8, 32, 8, 64, 640, 0, 1),
+    (16, 16, 8, 96, 600, 0, 1), (1, 6, 2, 32, 640, 0, 1), (8, 16, 8, 128, 641, 0, 3)])
+@pytest.mark.parametrize("even", [False, True])
+def test_somewhat_more_than_512_keys_go_by_what_was_timed(B, Hq, Hkv, D, ctx, span, pieces, even):
+    part, parts = ops.decode_partitions_e4m3(B, Hq, Hkv, ctx, span, even, D)
+    assert parts == pieces and (part == 256 or parts == 1)
+
+
 def test_nan_is_the_only_number_that_is_not_finite():
     x = torch.tensor([math.inf, -math.inf, math.nan, 1.0], dtype=torch.float64)
     assert torch.isnan(to_e4m3(x)).tolist() == [True, True, True, False]
