@@ -141,6 +141,63 @@ def test_generation_on_the_cpu(folders, plain):
     assert [len(o["token_ids"]) for o in outs] == [6, 6, 6] and all(len(o["token_ids"]) == 6 for o in again)
 
 
+def _evicted_and_refed(folder, vocab, lens, tokens, pages, **options):
+    """A pool that is too small for all requests: some are evicted and fed again, into blocks that others held before; a second run finds the first
+    one's full pages. Every token is the plain model's best, or lies within what 8 bits cost of it, and is the one that the request gets
+    alone in a cache of its own, up to a first place where the plain model's logits of the two lie as near to each other."""
+    prompts = [helpers.random_ids(n, vocab, 7 + n) for n in lens]
+    params = SamplingParams(temperature=0, max_tokens=tokens)
+    run = lambda llm, p: [o["token_ids"] for o in llm.generate(p, params, use_tqdm=False)]  # noqa: E731
+    tight = LLM(folder, num_kvcache_blocks=pages, kv_cache_dtype="e4m3", dtype="bfloat16", poison_cache=True, **options)
+    first = run(tight, prompts)
+    assert tight.scheduler.num_preemptions > 0, "nobody was evicted"
+    before = tight.scheduler.num_prefix_hits
+    again = run(tight, prompts)
+    assert tight.scheduler.num_prefix_hits > before, "no page was found again"
+    cfg, w = plain_qwen3.read_model_folder(folder, torch.float64)
+    for i, p in enumerate(prompts):
+        own = LLM(folder, num_kvcache_blocks=64, kv_cache_dtype="e4m3", dtype="bfloat16", poison_cache=True, enable_prefix_caching=False, **options)
+        alone = run(own, [p])[0]
+        assert own.scheduler.num_preemptions == 0 and len(alone) == tokens
+        for out in (first[i], again[i]):
+            assert len(out) == tokens
+            z = plain_qwen3.logits(cfg, w, p + out)
+            same = True
+            for j, tok in enumerate(out):
+                row = z[len(p) + j - 1]
+                near = 2 * 0.11 * 3 * _rms(row)           # two logits, each off by 0.11 of the logits' size on average (above), three times that at most
+                assert float(row.max() - row[tok]) <= near, (i, j)
+                if same and tok != alone[j]:
+                    assert abs(float(row[alone[j]] - row[tok])) <= near, (i, j)
+                    same = False
+
+
+def test_evicted_requests_on_the_cpu(folders, plain):
+    _evicted_and_refed(folders("A"), 256, (5, 37, 33), 20, 6, device="cpu", max_num_seqs=4, max_num_batched_tokens=32, max_model_len=64)
+
+
+# Configurations of the other designs: None where all their attention has the 8-bit form, else why they are refused.
+DESIGNS = {("sigosun_cases", n): None for n in ("mix", "odd", "att", "far", "real")} | {
+    ("goluzen_cases", "one"): None, ("tavevik_cases", "two"): None, ("goluzen_cases", "real"): "kept behind a window", ("goluzen_cases", "routed"): "cap",
+    ("tavevik_cases", "real"): "kept behind a window", ("tavevik_cases", "odd"): "kept behind a window", ("venezen_cases", "real"): "slopes",
+    ("venezen_cases", "windows"): "slopes", ("negosun_cases", "real"): "whole projections", ("vefulix_cases", "real"): "nothing to hold",
+    ("sigosun_cases", "ssm"): "nothing to hold"}
+
+
+@pytest.mark.parametrize("module,name", list(DESIGNS), ids=lambda x: x)
+def test_designs_that_have_the_form(tmp_path, module, name):
+    import importlib
+    model = load_model(importlib.import_module(module).make_folder(name, str(tmp_path / "model")), "cpu", torch.bfloat16, 64)
+    lacks = DESIGNS[module, name]
+    if lacks:
+        with pytest.raises(ValueError, match=lacks):
+            model.hold_keys_and_values_in("e4m3")
+        return
+    model.hold_keys_and_values_in("e4m3")
+    kept = [t.dtype for need in model.cache_plan().group_needs for t in need.tensors]
+    assert "e4m3" in kept and kept.count("e4m3") == kept.count("uint8")
+
+
 # ------------------------------------------------------------------ on the GPU
 
 @pytest.mark.gpu
@@ -211,3 +268,34 @@ def test_other_designs_on_the_gpu(tmp_path):
                 assert torch.isfinite(found["e4m3"][r]).all()
                 assert _rms(found["e4m3"][r] - found["compute"][r]) <= 0.3 * _rms(found["compute"][r])
     assert ran >= 1
+
+
+@pytest.mark.gpu
+def test_evicted_requests_on_the_gpu(folders):
+    """Captured steps, run ahead, beside portions: the blocks that a step writes ahead of a request's end are others' soon after."""
+    _evicted_and_refed(folders("R"), 2048, (5, 130, 33, 90), 40, 16, max_num_seqs=4, max_num_batched_tokens=64, max_model_len=256)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("module,name", [k for k, lacks in DESIGNS.items() if not lacks], ids=lambda x: x)
+def test_designs_steps_on_the_gpu(tmp_path, module, name):
+    """The kernels' steps against the plain forms' on the CPU. Two runs whose stored numbers were rounded with nothing to do with each
+    other would differ by sqrt(2) of what storing costs; bfloat16's roundings in front of the cache cannot take them further apart."""
+    import importlib
+    folder = importlib.import_module(module).make_folder(name, str(tmp_path / "model"))
+
+    def logits(kind, device):
+        model = load_model(folder, device, torch.bfloat16, 256)
+        model.hold_keys_and_values_in(kind)
+        manager = CacheManager(40, 16, ModelRunner.windows_of(model), num_state_slots=4, enable_prefix_caching=False)
+        ids, cuts = _requests(model.embedding.vocab_size)
+        return _feed(ModelRunner(model, manager, torch.bfloat16, device, 256, poison_cache=True), manager, ids, cuts)
+    got = logits("e4m3", "cuda")
+    ops.set_backend(Plain())
+    try:
+        expect, full = logits("e4m3", "cpu"), logits("compute", "cpu")
+    finally:
+        ops.set_backend(None)
+    for r in got:
+        assert torch.isfinite(got[r]).all()
+        assert _rms(got[r] - expect[r]) <= 2 ** 0.5 * _rms(expect[r] - full[r]) + helpers.TOL_BF16 * _rms(full[r])
