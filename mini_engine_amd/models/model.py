@@ -63,14 +63,17 @@ class DecoderModel(Part):
     def hold_keys_and_values_in(self, kind: str) -> None:
         """`kind`: what the attention layers' pages hold, "compute" (the engine's data type) or "e4m3" (8 bits under a power of two per
         16 tokens and head). Other mixers keep what they keep. Raises ValueError where a layer's attention has no such form, or where
-        no layer keeps keys and values. Before the cache is made."""
+        no layer keeps keys and values, and leaves every layer as it was. Before the cache is made."""
         holders = [(i, part) for i, layer in enumerate(self.layers) for part in layer.parts() if hasattr(part, "hold_in")]
         if kind != "compute" and not holders:
             raise ValueError("no layer of this model keeps keys and values: there is nothing to hold in 8 bits")
+        before = [getattr(mixer, "pages_hold", "compute") for _, mixer in holders]
         for i, mixer in holders:
             try:
                 mixer.hold_in(kind)
             except ValueError as e:
+                for (_, earlier), held in zip(holders, before):
+                    earlier.hold_in(held)
                 raise ValueError(f"layer {i}: {e}") from None
 
     # -- what the cache has to provide ------------------------------------------------------

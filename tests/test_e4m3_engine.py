@@ -198,6 +198,17 @@ def test_designs_that_have_the_form(tmp_path, module, name):
     assert "e4m3" in kept and kept.count("e4m3") == kept.count("uint8")
 
 
+@pytest.mark.parametrize("name", ["pair", "real"])
+def test_a_refused_model_is_left_as_it_was(tmp_path, name):
+    """Tavevik's first attention layer has the form, its second one has not."""
+    import tavevik_cases
+    model = load_model(tavevik_cases.make_folder(name, str(tmp_path / "model")), "cpu", torch.bfloat16, 64)
+    before = model.cache_plan().group_needs
+    with pytest.raises(ValueError, match="layer 1: .*no keys kept behind a window"):
+        model.hold_keys_and_values_in("e4m3")
+    assert model.cache_plan().group_needs == before
+
+
 # ------------------------------------------------------------------ on the GPU
 
 @pytest.mark.gpu
