@@ -1,6 +1,8 @@
 // The write into the 8-bit cache (e4m3.h): per-head RMSNorm of q and k, rotation, and the scatter of k and v into their pages, in
 // one launch over the packed rows. q goes out as rows of its own, rounded to bfloat16 once; k and v are rounded to e4m3 once, from
-// the float32 results, and from exact ones where that could make a difference.
+// the float32 results (v is its row's number as it is). A key that lies within 8 float32 steps of the middle between two e4m3 numbers is
+// rounded from an exact result; what cancellation in the rotation leaves further off than that may still fall to the other side, and
+// a block's power goes by the float32 results.
 //
 //   k' = rotated(w * k / rms(k));  block (16 places of a page, head): p = max(p_before if places in front of the call's first
 //   place are held, least power with max |k'| <= 448 * 2^p);  stored: e4m3(k' 2^-p), numbers held before: e4m3(old 2^(p_before - p)).
