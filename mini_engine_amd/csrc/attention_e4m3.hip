@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attn8_decode_kernel(At
 // single weights instead of pairs cost 6%; registers of scores that change their meaning every second step instead of being copied, 2%.
 //
 // Bound by the matrix cores' and the vector units' shared issue: of 930 cycles a step and wave at 8,192 tokens 512 are products (55% of the
-// time; two waves to a unit) and 45% of a wave's time is issue. 470 us there are 1,170 TF/s, against 1,430 of a large bfloat16 product.
+// time; two waves to a unit) and 45% of a wave's time is issue. 478 us there are 1,150 TF/s, against 1,430 of a large bfloat16 product.
 // A workgroup alone on its unit takes 0.5 us a step, two of them 0.9, so a short prompt takes what its last tile takes: 2,048 tokens (16
 // heads over 8) 44 us, of which 5.5 until the first step. Two sets of 4 waves that share a tile's keys came to 41 us there and
 // cost portions of few tokens 3 us; 64 columns to a wave left one wave to a unit: 657 us for 590.

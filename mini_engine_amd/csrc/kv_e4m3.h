@@ -164,7 +164,7 @@ __device__ __forceinline__ int row_slot(const AppendArgs& a, int64_t t) {
 
 // Whether a number, scaled for its block, lies so near to the middle between two e4m3 numbers that float32 may have put it on the other side:
 // within 8 of its steps. There it would be off by a whole step of e4m3 (one number in 650,000 was, most of them by one of the large
-// steps; what cancellation leaves further off is small, and so are its steps); one in 65,000 is done again by norm_rotate_key. 60 rows
+// steps; what cancellation leaves further off is small, and so are its steps); one in 65,000 is done again by norm_rotate_key. 64 rows
 // of one token 6.4 us in float32 alone, 8.4 so; 7,900 rows of 32 and 8 heads of 128 48.5 and 49.6 (53 where the queries' waves have 132
 // registers instead of 128), with every key done so 59, all in double 66.
 __device__ __forceinline__ bool between(float x) { return ((__float_as_uint(x) + 0x80008u) & 0xfffffu) < 0x10u; }
